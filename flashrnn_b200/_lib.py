@@ -13,6 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libflashrnn_b200.so"
 
 CELLS = {"lstm": 0, "slstm": 1, "gru": 2, "elman": 3}
+LINEAR_CELLS = {"leaky": 0, "lstm": 1}
 
 ERROR_TEXT = {
     -1: "unknown cell",
@@ -73,6 +74,13 @@ class MgPlan(ctypes.Structure):
     ]
 
 
+class LinearPlan(ctypes.Structure):
+    """Mirror of ``frnn_b200_linear_plan_t``."""
+
+    _fields_ = [("gates", c_int), ("tile_steps", c_int), ("tile_channels", c_int), ("tiles", c_int),
+                ("exchange_bytes", c_int64), ("starts_bytes", c_int64), ("dbpart_bytes", c_int64)]
+
+
 # name -> (restype, argtypes); must list every function declared in include/flashrnn_b200.h
 SIGNATURES = {
     "frnn_b200_version": (c_int, []),
@@ -103,6 +111,12 @@ SIGNATURES = {
                                         c_int, c_void_p, c_void_p]),
     "frnn_b200_input_projection": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                            c_void_p, c_void_p]),
+    "frnn_b200_linear_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, POINTER(LinearPlan)]),
+    "frnn_b200_linear_forward": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "frnn_b200_linear_backward": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                          c_void_p, c_void_p]),
     "frnn_b200_mg_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, POINTER(MgShard), POINTER(MgPlan)]),
     "frnn_b200_mg_capacity": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "frnn_b200_mg_forward": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -171,6 +185,25 @@ def plan(cell: str, B: int, T: int, N: int, D: int, device: int = None) -> Plan:
     if len(_plans) > 4096:
         _plans.clear()
     _plans[key] = out
+    return out
+
+
+_linear_plans: dict = {}
+
+
+def linear_plan(function: str, B: int, T: int, N: int, D: int) -> LinearPlan:
+    """Scratch sizes of the gated linear recurrence, which depend on the shape only."""
+    key = (function, B, T, N, D)
+    hit = _linear_plans.get(key)
+    if hit is not None:
+        return hit
+    out = LinearPlan()
+    rc = load().frnn_b200_linear_plan(LINEAR_CELLS[function], B, T, N, D, ctypes.byref(out))
+    if rc != 0:
+        raise ValueError(f"frnn_b200_linear_plan failed: {ERROR_TEXT.get(rc, rc)}")
+    if len(_linear_plans) > 4096:
+        _linear_plans.clear()
+    _linear_plans[key] = out
     return out
 
 

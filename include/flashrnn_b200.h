@@ -213,6 +213,39 @@ int frnn_b200_input_projection(const void* x_bf16, const void* w_bf16, const flo
                                int T, int gates_times_width, int inputs, int* err, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Gated linear recurrence: no recurrent matrix, scanned in parallel over time. Per channel (head, unit), with
+ * x = Wx + b and gates in the order given:
+ *   leaky (f, z):        c_t = sigmoid(f) c_{t-1} + (1 - sigmoid(f)) z,            hidden = c
+ *   lstm  (i, f, z, o):  c_t = sigmoid(f) c_{t-1} + sigmoid(i) tanh(z),            hidden = sigmoid(o) tanh(c)
+ * wx [B,T,G,N,D], hidden and d_hidden [B,T,N,D], dwx [B,T,G,N,D]: bf16 (wx_bf16 = 1) or fp32, 16-byte aligned. Everything else
+ * is fp32: bias, db [G,N,D], initial, last, d_last, d_initial [B,N,D]. initial, d_last = NULL: zeros. lengths: int32 [B] (values
+ * are clamped to [0, T]) or NULL: steps at or behind a row's length leave its state alone, their hidden states and gradients
+ * are zero, whatever wx and d_hidden hold there. */
+enum { FRNN_LINEAR_LEAKY = 0, FRNN_LINEAR_LSTM = 1 };
+
+typedef struct frnn_b200_linear_plan {
+  int gates;
+  int tile_steps, tile_channels;  /* of one CTA                                                             */
+  int tiles;                      /* along time                                                             */
+  int64_t exchange_bytes;         /* scratch of either call, 16-byte aligned; 0: exchange and err may be NULL */
+  int64_t starts_bytes;           /* fp32 [B][tiles - 1][N][D], forward -> backward                         */
+  int64_t dbpart_bytes;           /* fp32 [B * tiles][G][N][D], scratch of the backward call                */
+} frnn_b200_linear_plan_t;
+
+int frnn_b200_linear_plan(int function, int B, int T, int N, int D, frnn_b200_linear_plan_t* out);
+
+/* starts: NULL for inference, or where plan.starts_bytes is 0. With one tile `last` may be `initial`. A wait that runs out
+ * (exchange_bytes > 0) is reported through err as 106. */
+int frnn_b200_linear_forward(int function, const void* wx, int wx_bf16, const float* bias, const float* initial, const int* lengths,
+                             void* hidden, float* last, float* starts, void* exchange, int B, int T, int N, int D, int wait_limit_ms,
+                             int* err, void* stream);
+
+/* d_initial may be NULL. */
+int frnn_b200_linear_backward(int function, const void* wx, int wx_bf16, const float* bias, const float* initial, const int* lengths,
+                              const float* starts, const void* d_hidden, const float* d_last, void* dwx, float* db, float* d_initial,
+                              float* db_part, void* exchange, int B, int T, int N, int D, int wait_limit_ms, int* err, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * One WIDE head (N = 1, D a multiple of 256) whose recurrent matrix is split over P GPUs of a node:
  * rank r owns the hidden units [r*Dl, (r+1)*Dl), Dl = D/P (a multiple of 128): the rows R[g, o in slice, :] in the
  * forward pass and the columns R[g, :, p in slice] in the backward pass; the per-step operand (round_bf16(h_t),
