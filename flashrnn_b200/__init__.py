@@ -7,7 +7,7 @@ Public surface = the reference's: ``flashrnn``, ``FlashRNNConfig``, ``flashrnn_t
 from .functional import BACKEND, SIZES, FlashRNNConfig, flashrnn, flashrnn_torch, poll_errors
 from .linear import flashrnn_linear
 from .prepared import PreparedSequence
-from .projection import flashrnn_projected, input_projection
+from .projection import flashrnn_projected, fused_projection, input_projection
 
 __all__ = ["BACKEND", "SIZES", "FlashRNNConfig", "PreparedSequence", "flashrnn", "flashrnn_linear", "flashrnn_projected",
-           "flashrnn_torch", "input_projection", "poll_errors"]
+           "flashrnn_torch", "fused_projection", "input_projection", "poll_errors"]

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libflashrnn_b200.so"
 
 CELLS = {"lstm": 0, "slstm": 1, "gru": 2, "elman": 3}
 LINEAR_CELLS = {"leaky": 0, "lstm": 1}
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
 
 ERROR_TEXT = {
     -1: "unknown cell",
@@ -81,6 +82,12 @@ class LinearPlan(ctypes.Structure):
                 ("exchange_bytes", c_int64), ("starts_bytes", c_int64), ("dbpart_bytes", c_int64)]
 
 
+class ProductPlan(ctypes.Structure):
+    """Mirror of ``frnn_b200_product_plan_t``."""
+
+    _fields_ = [("forward_work_bytes", c_int64), ("backward_work_bytes", c_int64), ("dbpart_bytes", c_int64)]
+
+
 # name -> (restype, argtypes); must list every function declared in include/flashrnn_b200.h
 SIGNATURES = {
     "frnn_b200_version": (c_int, []),
@@ -117,6 +124,11 @@ SIGNATURES = {
     "frnn_b200_linear_backward": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                           c_void_p, c_void_p]),
+    "frnn_b200_product_plan": (c_int, [c_int64, c_int, c_int, POINTER(ProductPlan)]),
+    "frnn_b200_product_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64,
+                                          c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "frnn_b200_product_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                           c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "frnn_b200_mg_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, POINTER(MgShard), POINTER(MgPlan)]),
     "frnn_b200_mg_capacity": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "frnn_b200_mg_forward": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -204,6 +216,25 @@ def linear_plan(function: str, B: int, T: int, N: int, D: int) -> LinearPlan:
     if len(_linear_plans) > 4096:
         _linear_plans.clear()
     _linear_plans[key] = out
+    return out
+
+
+_product_plans: dict = {}
+
+
+def product_plan(rows: int, outputs: int, inputs: int, device: int) -> ProductPlan:
+    """Scratch sizes of the product with an epilogue on the current CUDA device, whose index is ``device``."""
+    key = (device, rows, outputs, inputs)
+    hit = _product_plans.get(key)
+    if hit is not None:
+        return hit
+    out = ProductPlan()
+    rc = load().frnn_b200_product_plan(rows, outputs, inputs, ctypes.byref(out))
+    if rc != 0:
+        raise ValueError(f"frnn_b200_product_plan failed: {ERROR_TEXT.get(rc, rc)}")
+    if len(_product_plans) > 4096:
+        _product_plans.clear()
+    _product_plans[key] = out
     return out
 
 

@@ -21,7 +21,7 @@ LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libflashrnn_b200.so"
 SOURCES = ("capi.cu", "capi_mg.cu", *(f"recurrent_{k}_{c}.cu" for k in ("reg_bwd", "reg_fwd", "wide_bwd", "wide_fwd") for c in ("slstm", "lstm", "gru", "elman")),
            "recurrent_fwd.cu", "recurrent_fwd_ksplit.cu", "recurrent_bwd.cu", "recurrent_bwd_ksplit.cu",
-           "recurrent_mg_fwd.cu", "recurrent_mg_bwd.cu", "wgrad.cu", "input_proj.cu", "linear_scan.cu")
+           "recurrent_mg_fwd.cu", "recurrent_mg_bwd.cu", "wgrad.cu", "input_proj.cu", "linear_scan.cu", "product.cu")
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC",

@@ -1,0 +1,671 @@
+// Matrix product with an epilogue, y = act(x W^T + bias) + residual, and its gradients. bf16 operands, fp32 accumulation in tensor
+// memory, one rounding where a result is stored.
+//
+//   forward  y  [rows][outputs] : x  [rows][inputs]  (K-major)  . W  [outputs][inputs] (K-major),  K = inputs
+//            z = x W^T + bias is kept for the backward pass where the activation's slope needs it: as fp16, which has 11
+//            significant bits of it (the slope then is off by a few 2^-12; the gradients that it scales are rounded to the 8 bits of
+//            bf16) and takes half the room of fp32; values past 65504, where slopes are 0 or 1, are held at 65504
+//   dz = dy act'(z), rounded to bf16 for the tensor cores; dbias sums it before that rounding
+//   dx [rows][inputs]           : dz [rows][outputs] (K-major)  . W                    (MN-major), K = outputs
+//   dW [outputs][inputs]        : dz                 (MN-major) . x                    (MN-major), K = rows
+//
+// product_kernel: persistent, one CTA pair (cluster of two, cta_group::2) per two SMs, each pair walking 256 x NP output tiles.
+// A CTA stages its 128 rows of A and half of the NP rows of B, so that a pair moves 32 KB per CTA and 64 k's where two
+// single CTAs with 128 x 256 tiles move 48. Warp 8 feeds the ring by TMA (128-byte swizzle), one thread of the even CTA issues
+// the MMAs of both, 8 warps of each CTA take the accumulator out of tensor memory: two accumulators, so the epilogue of a tile
+// runs under the contraction of the next. Rows and columns past the edges are read as zeros and not stored.
+// Few tiles with a long K are cut along K: partial tiles in fp32, summed in order by product_join_kernel, which then has the epilogue.
+#include "../../include/flashrnn_b200.h"
+
+#include "frnn_common.cuh"
+
+namespace frnn {
+
+namespace {
+
+constexpr int kThreads = 320;    // warps 0-7 epilogue, 8 TMA, 9 MMA
+constexpr int kEpiWarps = 8;
+constexpr int kStages = 4;
+constexpr int kKC = 64;          // k's per stage: 128 bytes of bf16, one swizzle row
+constexpr int kBufBytes = 4096;  // staging: 32 rows x 128 bytes
+constexpr int kSmem = kStages * 32768 + kEpiWarps * 3 * kBufBytes + 1024;
+constexpr uint64_t kLimit = 2000000000ull;
+
+struct ProductParams {
+  const void* bias;  // [N] or null
+  int* err;
+  int bias_bf16, act, has_residual, has_z;
+  int M, N, K;       // of the contraction
+  int n_mt, n_nt, chunks, chunks_per_split;
+  long long n_tiles;
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+// Both CTAs of the pair take part in these, one warp each.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D (256 x N over both CTAs' tensor memory) (+)= A (128 rows from each CTA) B (N / 2 rows from each); one thread of the even CTA.
+__device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once every MMA issued so far has completed.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair_here(uint32_t bar) {  // ... of this CTA only
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void ld_shared_v4(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t a, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  a = fabsf(a) > 65504.0f ? copysignf(65504.0f, a) : a;  // a NaN stays one
+  b = fabsf(b) > 65504.0f ? copysignf(65504.0f, b) : b;
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// silu and the tanh form of gelu are both z sigmoid(w(z)): z and sqrt(8 / pi) (z + 0.044715 z^3).
+constexpr float kGelu = 1.5957691216057308f, kGeluCube = 0.044715f;
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == FRNN_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  if constexpr (ACT == FRNN_ACT_SILU) return z * sigmoid_p(z);
+  if constexpr (ACT == FRNN_ACT_GELU_TANH) return z * sigmoid_p(kGelu * z * fmaf(kGeluCube * z, z, 1.0f));
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == FRNN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == FRNN_ACT_SILU) {
+    const float s = sigmoid_p(z);
+    return fmaf(z * s, 1.0f - s, s);
+  }
+  if constexpr (ACT == FRNN_ACT_GELU_TANH) {
+    const float s = sigmoid_p(kGelu * z * fmaf(kGeluCube * z, z, 1.0f));
+    return fmaf(z * s * (1.0f - s), kGelu * fmaf(3.0f * kGeluCube * z, z, 1.0f), s);
+  }
+  return 1.0f;
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void act_row(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = act_value<ACT>(v[i]);
+}
+template <int N>
+__device__ __forceinline__ void act_row(int act, float (&v)[N]) {
+  if (act == FRNN_ACT_RELU) act_row<FRNN_ACT_RELU>(v);
+  else if (act == FRNN_ACT_SILU) act_row<FRNN_ACT_SILU>(v);
+  else if (act == FRNN_ACT_GELU_TANH) act_row<FRNN_ACT_GELU_TANH>(v);
+}
+// What the slope is taken at. Of a relu the side of zero alone counts, which a small z could lose in 16 bits.
+__device__ __forceinline__ void keep_slope(int act, const float (&v)[8], float (&z)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = act == FRNN_ACT_RELU ? (v[i] > 0.0f ? 1.0f : 0.0f) : v[i];
+}
+// v[i] += bias[j + i], eight columns of a row of N (a multiple of eight)
+__device__ __forceinline__ void add_bias(const ProductParams& p, int j, float (&v)[8]) {
+  if (p.bias == nullptr || j >= p.N) return;
+  if (p.bias_bf16) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + j));
+    v[0] += bf16_lo(w.x); v[1] += bf16_hi(w.x); v[2] += bf16_lo(w.y); v[3] += bf16_hi(w.y);
+    v[4] += bf16_lo(w.z); v[5] += bf16_hi(w.z); v[6] += bf16_lo(w.w); v[7] += bf16_hi(w.w);
+  } else {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + j));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + j + 4));
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+}
+__device__ __forceinline__ void add_bf16(const uint32_t (&w)[4], float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+}
+
+// A_MN / B_MN: the operand's rows in memory run along M / N instead of K. PARTIAL: fp32 tiles of one of several parts of K, no epilogue.
+template <bool A_MN, bool B_MN, int NP, bool PARTIAL>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
+               const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
+               const __grid_constant__ CUtensorMap z_map) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2], s_done;
+  __shared__ __align__(8) uint64_t s_res[kEpiWarps][2];
+  __shared__ uint32_t s_tmem_base;
+  constexpr int NH = NP / 2;  // rows of B in each CTA
+  constexpr uint32_t kStageBytes = 16384u + NH * 128u, kCols = 2u * NP;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = static_cast<int>(cluster_rank());  // 0: the one that issues
+  const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the same offset in both CTAs
+  const uint32_t staging = base + kStages * kStageBytes;
+  const volatile int* abort_flag = p.err;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&s_full[s]), 1);
+      mbar_init(smem_u32(&s_empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&s_acc_full[a]), 1);
+      mbar_init(smem_u32(&s_acc_empty[a]), 2 * kEpiWarps);  // the epilogue warps of both CTAs, in the even one
+    }
+    for (int w = 0; w < kEpiWarps; ++w)
+      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
+    mbar_init(smem_u32(&s_done), 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc_pair(smem_u32(&s_tmem_base), kCols);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tbase = s_tmem_base;
+
+  // tile -> rows, columns, part of K
+  struct Tile { int m0, n0, split, c_begin, c_end; };
+  auto tile_at = [&](long long t) {
+    Tile r;
+    r.n0 = static_cast<int>(t % p.n_nt) * NP;
+    t /= p.n_nt;
+    r.m0 = static_cast<int>(t % p.n_mt) * 256;
+    r.split = static_cast<int>(t / p.n_mt);
+    r.c_begin = r.split * p.chunks_per_split;
+    r.c_end = min(r.c_begin + p.chunks_per_split, p.chunks);
+    return r;
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      tma_prefetch_desc(&a_map);
+      tma_prefetch_desc(&b_map);
+      uint32_t s = 0, round = 0;
+      bool dead = false;
+      for (long long t = pair; t < p.n_tiles && !dead; t += pairs) {
+        const Tile tile = tile_at(t);
+        const int ma = tile.m0 + 128 * cta, nb = tile.n0 + NH * cta;
+        for (int i = tile.c_begin; i < tile.c_end; ++i) {
+          if (round > 0 && !mbar_wait_bounded<true, true>(smem_u32(&s_empty[s]), (round - 1) & 1, kLimit, abort_flag)) {
+            atomicCAS(p.err, 0, kErrWaitEmpty);
+            dead = true;
+            break;
+          }
+          const uint32_t bar = map_to_cta(smem_u32(&s_full[s]), 0);
+          const uint32_t sa = base + s * kStageBytes, sb = sa + 16384u;
+          if (cta == 0) mbar_arrive_expect_tx(smem_u32(&s_full[s]), 2 * kStageBytes);  // what both CTAs stage
+          const int k0 = i * kKC;
+          if constexpr (A_MN) {
+            tma_load_2d_pair(sa, &a_map, bar, ma, k0);
+            tma_load_2d_pair(sa + 8192u, &a_map, bar, ma + 64, k0);
+          } else {
+            tma_load_2d_pair(sa, &a_map, bar, k0, ma);
+          }
+          if constexpr (B_MN) {
+            for (int j = 0; j < NH / 64; ++j) tma_load_2d_pair(sb + j * 8192u, &b_map, bar, nb + 64 * j, k0);
+          } else {
+            tma_load_2d_pair(sb, &b_map, bar, k0, nb);
+          }
+          if (++s == kStages) { s = 0; ++round; }
+        }
+      }
+      // the last arrivals on this CTA's barriers are in before it leaves
+      for (uint32_t left = round > 0 ? kStages : s; left > 0 && !dead; --left) {
+        const uint32_t r = s > 0 ? round : round - 1;
+        s = s > 0 ? s - 1 : kStages - 1;
+        round = r;
+        dead = !mbar_wait_bounded<true, true>(smem_u32(&s_empty[s]), r & 1, kLimit, abort_flag);
+        if (dead) atomicCAS(p.err, 0, kErrWaitEmpty);
+      }
+      if (dead) {  // copies in flight land before the CTA leaves
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && cta == 0) {
+      const uint32_t idesc = umma_idesc_bf16(256, NP, A_MN, B_MN);
+      uint32_t s = 0, round = 0, li = 0;
+      bool dead = false;
+      for (long long t = pair; t < p.n_tiles && !dead; t += pairs, ++li) {
+        const Tile tile = tile_at(t);
+        const uint32_t a = li & 1u;
+        if (li >= 2 && !mbar_wait_bounded<true, true>(smem_u32(&s_acc_empty[a]), ((li >> 1) - 1) & 1, kLimit, abort_flag)) {
+          atomicCAS(p.err, 0, kErrWaitEpi);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t d = tbase + a * NP;
+        for (int i = tile.c_begin; i < tile.c_end; ++i) {
+          if (!mbar_wait_bounded<true, true>(smem_u32(&s_full[s]), round & 1, kLimit, abort_flag)) {
+            atomicCAS(p.err, 0, kErrWaitWx);
+            dead = true;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = base + s * kStageBytes, sb = sa + 16384u;
+          // 16 k's further: 32 bytes inside the swizzled row, or 16 rows of 128 bytes
+          uint64_t ad = A_MN ? umma_smem_desc_mn_sw128(sa, 8192u) : umma_smem_desc_k_sw128(sa);
+          uint64_t bd = B_MN ? umma_smem_desc_mn_sw128(sb, 8192u) : umma_smem_desc_k_sw128(sb);
+#pragma unroll
+          for (int kk = 0; kk < kKC / 16; ++kk) {
+            umma_bf16_pair(d, ad, bd, idesc, (i > tile.c_begin || kk > 0) ? 1u : 0u);
+            ad += A_MN ? 128 : 2;
+            bd += B_MN ? 128 : 2;
+          }
+          umma_commit_pair(smem_u32(&s_empty[s]));
+          if (++s == kStages) { s = 0; ++round; }
+        }
+        if (!dead) umma_commit_pair(smem_u32(&s_acc_full[a]));
+      }
+      // covers every MMA issued so far, also after a failed wait: tensor and shared memory stay until they are done
+      umma_commit_pair_here(smem_u32(&s_done));
+      mbar_wait_bounded<true, true>(smem_u32(&s_done), 0, kLimit, nullptr);
+    }
+  } else {
+    const int q = warp & 3, half = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; columns
+    constexpr int CW = PARTIAL ? 32 : 64;      // columns of a piece: 128 bytes
+    constexpr int kPieces = NH / CW;           // a warp has half of the tile's NP columns
+    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 3u * kBufBytes, zbuf = buf0 + 2u * kBufBytes;
+    const uint32_t my_row = static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
+    uint32_t li = 0, used = 0, res_phase = 0;  // used: pieces staged so far; res_phase: a bit per buffer
+    for (long long t = pair; t < p.n_tiles; t += pairs, ++li) {
+      const Tile tile = tile_at(t);
+      const uint32_t a = li & 1u;
+      const int mw = tile.m0 + 128 * cta + 32 * q, j0 = tile.n0 + NH * half;
+      const bool any = mw < p.M && j0 < p.N;   // warp-uniform
+      if constexpr (!PARTIAL) {
+        if (p.has_residual && any && lane == 0) {  // both pieces, while the tensor cores work
+          tma_store_wait_read<0>();
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            if (j0 + i * CW >= p.N) break;
+            const uint32_t bi = (used + i) & 1u, bar = smem_u32(&s_res[warp][bi]);
+            mbar_arrive_expect_tx(bar, kBufBytes);
+            tma_load_2d(buf0 + bi * kBufBytes, &res_map, bar, j0 + i * CW, mw);
+          }
+        }
+      }
+      const bool have = mbar_wait_warp<true>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag);
+      if (!have) {
+        if (lane == 0) atomicCAS(p.err, 0, kErrWaitMma);
+        break;
+      }
+      tc_fence_after_sync();
+#pragma unroll 1
+      for (int i = 0; i < kPieces; ++i) {
+        const int c = a * NP + NH * half + i * CW, j = j0 + i * CW;
+        uint32_t r[CW];
+        tmem_ld_x32(tmem_addr(tbase, 32 * q, c), *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        if constexpr (CW == 64) tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tmem_ld_wait();
+        if (i == kPieces - 1) {  // the accumulator is in registers: the next tile but one may have it
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s_acc_empty[a]), 0));
+        }
+        if (!any || j >= p.N) continue;
+        const uint32_t bi = used & 1u, buf = buf0 + bi * kBufBytes;
+        ++used;
+        if constexpr (PARTIAL) {
+          if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t w[4] = {r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]};
+            st_shared_v4(buf + my_row + ((k ^ sw) << 4), w);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&out_map, buf, j, mw, tile.split);
+            tma_store_commit();
+          }
+        } else {
+          if (p.has_residual) {
+            if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][bi]), (res_phase >> bi) & 1u, kLimit, abort_flag)) {
+              if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
+            }
+            res_phase ^= 1u << bi;
+            if (p.has_z && lane == 0) tma_store_wait_read<0>();
+          } else if (lane == 0) {
+            if (p.has_z) tma_store_wait_read<0>();
+            else tma_store_wait_read<1>();
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t at = my_row + ((k ^ sw) << 4);
+            float v[8], zv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[8 * k + e]);
+            add_bias(p, j + 8 * k, v);
+            if (p.has_z) {
+              keep_slope(p.act, v, zv);
+              const uint32_t w[4] = {pack_half2(zv[0], zv[1]), pack_half2(zv[2], zv[3]), pack_half2(zv[4], zv[5]), pack_half2(zv[6], zv[7])};
+              st_shared_v4(zbuf + at, w);
+            }
+            act_row(p.act, v);
+            if (p.has_residual) {
+              uint32_t w[4];
+              ld_shared_v4(buf + at, w);
+              add_bf16(w, v);
+            }
+            const uint32_t w[4] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+            st_shared_v4(buf + at, w);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&out_map, buf, j, mw);
+            if (p.has_z) tma_store_2d(&z_map, zbuf, j, mw);
+            tma_store_commit();
+          }
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait<0>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the other CTA's operands, barriers and tensor memory are in use until here
+  if (warp == 9) tmem_dealloc_pair(tbase, kCols);
+}
+
+// out = epilogue(sum over parts of work), eight columns of a row to a thread.
+__global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p, const float* __restrict__ work, int parts,
+                                                           const __nv_bfloat16* __restrict__ residual, __nv_bfloat16* __restrict__ out,
+                                                           __half* __restrict__ z) {
+  const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 8, n = static_cast<long long>(p.M) * p.N;
+  if (i >= n) return;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  for (int s = 0; s < parts; ++s) {
+    float w[8];
+    ld_f32_vec<8>(work + s * n + i, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += w[e];
+  }
+  add_bias(p, static_cast<int>(i % p.N), v);
+  if (z != nullptr) {
+    float zv[8];
+    keep_slope(p.act, v, zv);
+    *reinterpret_cast<uint4*>(z + i) =
+        make_uint4(pack_half2(zv[0], zv[1]), pack_half2(zv[2], zv[3]), pack_half2(zv[4], zv[5]), pack_half2(zv[6], zv[7]));
+  }
+  act_row(p.act, v);
+  if (residual != nullptr) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(residual + i));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    add_bf16(w, v);
+  }
+  *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// dz = dy act'(z) (not stored where the activation is none: dz = dy), and the columns' sums of a block's rows for dbias.
+constexpr int kSlopeRows = 64;
+template <int ACT>
+__global__ void __launch_bounds__(256) product_slope_kernel(const __nv_bfloat16* __restrict__ dy, const __half* __restrict__ z,
+                                                            __nv_bfloat16* __restrict__ dz, float* __restrict__ part, int M, int N) {
+  __shared__ float s_sum[8][32][9];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.y * 32 + lane) * 8;
+  const int m_end = min((static_cast<int>(blockIdx.x) + 1) * kSlopeRows, M);
+  float sum[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+  if (j < N) {
+#pragma unroll 4
+    for (int m = blockIdx.x * kSlopeRows + warp; m < m_end; m += 8) {
+      const long long at = static_cast<long long>(m) * N + j;
+      const uint4 g = __ldg(reinterpret_cast<const uint4*>(dy + at));
+      float v[8] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y), bf16_lo(g.z), bf16_hi(g.z), bf16_lo(g.w), bf16_hi(g.w)};
+      if constexpr (ACT != FRNN_ACT_NONE) {
+        const uint4 h = __ldg(reinterpret_cast<const uint4*>(z + at));
+        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+          v[2 * e] *= act_slope<ACT>(f.x);
+          v[2 * e + 1] *= act_slope<ACT>(f.y);
+        }
+        *reinterpret_cast<uint4*>(dz + at) =
+            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s_sum[warp][lane][e] = sum[e];
+  __syncthreads();
+  const int l = threadIdx.x >> 3, e = threadIdx.x & 7, col = (blockIdx.y * 32 + l) * 8 + e;
+  if (col < N) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += s_sum[w][l][e];
+    part[static_cast<long long>(blockIdx.x) * N + col] = v;
+  }
+}
+
+// out[j] = sum over rows of part[row][j], in a fixed order.
+__global__ void __launch_bounds__(1024) product_bias_kernel(const float* __restrict__ part, void* __restrict__ out, int out_bf16, int rows, int cols) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+  float sum = 0.0f;
+  if (j < cols)
+    for (int r = warp; r < rows; r += 32) sum += part[static_cast<long long>(r) * cols + j];
+  s[warp][lane] = sum;
+  __syncthreads();
+  float v = s[lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int col = blockIdx.x * 32 + warp;
+  if (lane == 0 && col < cols) {
+    if (out_bf16) static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(v);
+    else static_cast<float*>(out)[col] = v;
+  }
+}
+
+// How an M x N x K product is cut: columns of a tile, parts of K.
+struct Cut { int np, parts, chunks_per_part; };
+Cut choose_cut(long long M, long long N, long long K) {
+  const long long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, mt = (M + 255) / 256, chunks = (K + kKC - 1) / kKC;
+  Cut best{};
+  double best_t = 0;
+  for (int np = 256; np >= 128; np /= 2) {
+    const long long tiles = mt * ((N + np - 1) / np);
+    for (long long parts = 1; parts <= 16 && parts <= chunks; ++parts) {
+      const long long cpp = (chunks + parts - 1) / parts;
+      if ((chunks + cpp - 1) / cpp != parts) continue;
+      const long long waves = (tiles * parts + pairs - 1) / pairs;
+      // cycles: 64 k's of a tile, filling and draining, the pass over partial sums (4 bytes written and read)
+      double t = static_cast<double>(waves) * cpp * (np == 256 ? 520 : 300) + 3000;
+      if (parts > 1) t += 5000 + static_cast<double>(M) * N * parts * 8 / 2500;
+      if (best.np == 0 || t < best_t) {
+        best = {np, static_cast<int>(parts), static_cast<int>(cpp)};
+        best_t = t;
+      }
+    }
+  }
+  return best;
+}
+long long work_bytes(long long M, long long N, long long K) {
+  const Cut c = choose_cut(M, N, K);
+  return c.parts > 1 ? 4 * M * N * c.parts : 0;
+}
+
+int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long long rows, uint32_t box_cols, uint32_t box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const uint32_t box[2] = {box_cols, box_rows};
+  return make_tensor_map(map, base, elem, 2, dims, box, true);
+}
+
+template <bool A_MN, bool B_MN, int NP, bool PARTIAL>
+int launch_kernel(const ProductParams& p, const CUtensorMap (&maps)[5], cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, PARTIAL>);
+  cudaError_t e = raise_limits(kern, kSmem, false);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const long long pairs = sm_count() / 2;
+  const unsigned grid = 2u * static_cast<unsigned>(p.n_tiles < pairs ? p.n_tiles : pairs);
+  product_kernel<A_MN, B_MN, NP, PARTIAL><<<grid, kThreads, kSmem, s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// C [M][N] = A . B with the epilogue of `p` (bias, act); A [M][K] or, A_MN, [K][M]; B [N][K] or, B_MN, [K][N].
+template <bool A_MN, bool B_MN>
+int product_launch(ProductParams p, const void* A, const void* B, long long M, long long N, long long K, const void* residual, void* out,
+                   void* z, float* work, cudaStream_t s) {
+  const Cut cut = choose_cut(M, N, K);
+  p.M = static_cast<int>(M); p.N = static_cast<int>(N); p.K = static_cast<int>(K);
+  p.n_mt = static_cast<int>((M + 255) / 256); p.n_nt = static_cast<int>((N + cut.np - 1) / cut.np);
+  p.chunks = static_cast<int>((K + kKC - 1) / kKC); p.chunks_per_split = cut.chunks_per_part;
+  p.n_tiles = static_cast<long long>(p.n_mt) * p.n_nt * cut.parts;
+  p.has_residual = residual != nullptr; p.has_z = z != nullptr;
+  CUtensorMap maps[5];
+  const uint32_t half = static_cast<uint32_t>(cut.np / 2);
+  int rc = A_MN ? map_2d(&maps[0], A, 2, M, K, 64, kKC) : map_2d(&maps[0], A, 2, K, M, kKC, 128);
+  if (rc == 0) rc = B_MN ? map_2d(&maps[1], B, 2, N, K, 64, kKC) : map_2d(&maps[1], B, 2, K, N, kKC, half);
+  if (rc != 0) return rc;
+  if (cut.parts > 1) {
+    if (work == nullptr) return -5;
+    const uint64_t dims[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(cut.parts)};
+    const uint32_t box[3] = {32, 32, 1};
+    rc = make_tensor_map(&maps[2], work, 4, 3, dims, box, true);
+    if (rc != 0) return rc;
+    maps[3] = maps[4] = maps[2];
+    rc = cut.np == 256 ? launch_kernel<A_MN, B_MN, 256, true>(p, maps, s) : launch_kernel<A_MN, B_MN, 128, true>(p, maps, s);
+    if (rc != 0) return rc;
+    const long long threads = M * N / 8;
+    product_join_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p, work, cut.parts, static_cast<const __nv_bfloat16*>(residual),
+                                                                                   static_cast<__nv_bfloat16*>(out), static_cast<__half*>(z));
+    return static_cast<int>(cudaGetLastError());
+  }
+  rc = map_2d(&maps[2], out, 2, N, M, 64, 32);
+  if (rc == 0 && residual != nullptr) rc = map_2d(&maps[3], residual, 2, N, M, 64, 32);
+  if (rc == 0 && z != nullptr) rc = map_2d(&maps[4], z, 2, N, M, 64, 32);
+  if (rc != 0) return rc;
+  if (residual == nullptr) maps[3] = maps[2];
+  if (z == nullptr) maps[4] = maps[2];
+  return cut.np == 256 ? launch_kernel<A_MN, B_MN, 256, false>(p, maps, s) : launch_kernel<A_MN, B_MN, 128, false>(p, maps, s);
+}
+
+bool bad_sizes(int64_t rows, int outputs, int inputs) { return rows < 1 || outputs < 1 || inputs < 1; }
+bool unsupported(int64_t rows, int outputs, int inputs) {
+  // coordinates and tile counts are 32-bit; 16-byte rows
+  return rows > 0x7fffff00LL || outputs > 0x7fffff00 || inputs > 0x7fffff00 || outputs % 8 != 0 || inputs % 8 != 0 ||
+         rows * outputs / 8 > 0x7fffffffLL * 256 || static_cast<long long>(inputs) * outputs / 8 > 0x7fffffffLL * 256;
+}
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool bad_act(int a) { return a != FRNN_ACT_NONE && a != FRNN_ACT_RELU && a != FRNN_ACT_SILU && a != FRNN_ACT_GELU_TANH; }
+
+}  // namespace
+
+}  // namespace frnn
+
+extern "C" int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frnn_b200_product_plan_t* out) {
+  using namespace frnn;
+  if (out == nullptr || bad_sizes(rows, outputs, inputs)) return -5;
+  if (unsupported(rows, outputs, inputs)) return -2;
+  *out = {};
+  out->forward_work_bytes = work_bytes(rows, outputs, inputs);
+  const long long dx = work_bytes(rows, inputs, outputs), dw = work_bytes(outputs, inputs, rows);
+  out->backward_work_bytes = dx > dw ? dx : dw;
+  out->dbpart_bytes = 4 * ((rows + kSlopeRows - 1) / kSlopeRows) * outputs;
+  return 0;
+}
+
+extern "C" int frnn_b200_product_forward(const void* x, const void* w, const void* bias, int bias_bf16, const void* residual, int activation,
+                                         void* y, void* z, int64_t rows, int outputs, int inputs, float* work, int* err, void* stream) {
+  using namespace frnn;
+  if (!x || !w || !y || !err || bad_sizes(rows, outputs, inputs) || bad_act(activation)) return -5;
+  if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias) || misaligned(residual) || misaligned(z) || misaligned(work)) return -5;
+  if (unsupported(rows, outputs, inputs)) return -2;
+  ProductParams p{};
+  p.bias = bias; p.bias_bf16 = bias_bf16; p.act = activation; p.err = err;
+  return product_launch<false, false>(p, x, w, rows, outputs, inputs, residual, y, z, work, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int frnn_b200_product_backward(const void* dy, const void* z, const void* x, const void* w, int activation, void* dz, void* dx,
+                                          void* dw, void* dbias, int dbias_bf16, float* db_part, int64_t rows, int outputs, int inputs,
+                                          float* work, int* err, void* stream) {
+  using namespace frnn;
+  const bool slopes = activation != FRNN_ACT_NONE;
+  if (!dy || !err || bad_sizes(rows, outputs, inputs) || bad_act(activation)) return -5;
+  if ((slopes && (!z || !dz)) || (dx && !w) || (dw && !x) || (dbias && !db_part)) return -5;
+  if (misaligned(dy) || misaligned(z) || misaligned(x) || misaligned(w) || misaligned(dz) || misaligned(dx) || misaligned(dw) ||
+      misaligned(work))
+    return -5;
+  if (unsupported(rows, outputs, inputs)) return -2;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (slopes || dbias != nullptr) {
+    const int blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows), cols = (outputs / 8 + 31) / 32;
+    if (cols > 65535) return -2;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(cols));
+    const auto* g = static_cast<const __nv_bfloat16*>(dy);
+    const auto* h = static_cast<const __half*>(z);
+    auto* d = static_cast<__nv_bfloat16*>(dz);
+    float* part = dbias != nullptr ? db_part : nullptr;
+    const int M = static_cast<int>(rows);
+    if (activation == FRNN_ACT_RELU) product_slope_kernel<FRNN_ACT_RELU><<<grid, 256, 0, s>>>(g, h, d, part, M, outputs);
+    else if (activation == FRNN_ACT_SILU) product_slope_kernel<FRNN_ACT_SILU><<<grid, 256, 0, s>>>(g, h, d, part, M, outputs);
+    else if (activation == FRNN_ACT_GELU_TANH) product_slope_kernel<FRNN_ACT_GELU_TANH><<<grid, 256, 0, s>>>(g, h, d, part, M, outputs);
+    else product_slope_kernel<FRNN_ACT_NONE><<<grid, 256, 0, s>>>(g, h, d, part, M, outputs);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && dbias != nullptr) {
+      product_bias_kernel<<<(outputs + 31) / 32, 1024, 0, s>>>(db_part, dbias, dbias_bf16, blocks, outputs);
+      e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  ProductParams p{};
+  p.err = err;
+  const void* g = slopes ? dz : dy;
+  int rc = 0;
+  if (dx != nullptr) rc = product_launch<false, true>(p, g, w, rows, inputs, outputs, nullptr, dx, nullptr, work, s);
+  if (rc == 0 && dw != nullptr) rc = product_launch<true, true>(p, g, x, outputs, inputs, rows, nullptr, dw, nullptr, work, s);
+  return rc;
+}

@@ -36,6 +36,12 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on the 16-byte boundary that the kernels' vector accesses need (a view may start anywhere)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 

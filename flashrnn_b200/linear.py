@@ -19,16 +19,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .functional import _error_word, _ptr, _stream, _track, poll_errors
+from .functional import _dense, _error_word, _ptr, _stream, _track, poll_errors
 
 # function -> gates of Wx and b
 LINEAR_GATES = {"leaky": 2, "lstm": 4}
-
-
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and on the 16-byte boundary that the kernels' vector accesses need (a view may start anywhere)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _scratch(plan, device):

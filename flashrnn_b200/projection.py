@@ -8,6 +8,10 @@ kernel (flashrnn/speed_experiments/kernel_speed_benchmark.py:388-408); ``W`` / `
 
 Backward of the projection (``dx = dWx @ W``, ``dW = dWx.T @ x``, ``dbias_w = sum dWx``) uses torch's library GEMMs: they
 are plain GEMMs with no recurrence-specific fusion to gain.
+
+``fused_projection(x, weight, bias, activation, residual)`` is the product around a recurrent layer with what surrounds it in the
+kernel's epilogue: the way into the gates, the way of the hidden states back into the residual stream, a feed-forward part. Its
+gradients run on this library's kernels.
 """
 
 from __future__ import annotations
@@ -15,9 +19,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .functional import SIZES, FlashRNNConfig, _error_word, _track, flashrnn, poll_errors
+from .functional import SIZES, FlashRNNConfig, _dense, _error_word, _ptr, _stream, _track, flashrnn, poll_errors
 
 
 class _Projection(torch.autograd.Function):
@@ -91,3 +96,122 @@ def flashrnn_projected(x, W, R, b, states=None, bias_w=None, function: str = "ls
     out_dtype = torch.bfloat16 if dtype == "bfloat16" else torch.float32
     wx = input_projection(x, W, bias_w, out_dtype).view(x.shape[0], x.shape[1], gw, N, D)
     return flashrnn(wx, R, b, states, function=function, config=config, dtype=dtype)
+
+
+def _product_forward(x, weight, bias, residual, activation, keep: bool):
+    """x [M,I], weight [J,I], residual [M,J] -> y [M,J] and, where the backward pass needs it, what the slope is taken at."""
+    lib = _lib.load()
+    poll_errors()
+    (M, I), J, dev = x.shape, weight.shape[0], x.device
+    plan = _lib.product_plan(M, J, I, dev.index)
+    y = torch.empty((M, J), dtype=torch.bfloat16, device=dev)
+    z = torch.empty((M, J), dtype=torch.float16, device=dev) if keep and activation is not None else None
+    work = torch.empty(plan.forward_work_bytes // 4, dtype=torch.float32, device=dev) if plan.forward_work_bytes else None
+    err = _error_word(dev)
+    rc = lib.frnn_b200_product_forward(
+        x.data_ptr(), weight.data_ptr(), _ptr(bias), int(bias is not None and bias.dtype == torch.bfloat16), _ptr(residual),
+        _lib.ACTIVATIONS[activation], y.data_ptr(), _ptr(z), M, J, I, _ptr(work), err.data_ptr(), _stream(dev))
+    _lib.check(rc, "frnn_b200_product_forward")
+    _track(err, "frnn_b200_product_forward")
+    return y, z
+
+
+class _FusedProjection(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, z = _product_forward(x, weight, bias, residual, activation, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None, z)
+        ctx.activation, ctx.sizes = activation, (*x.shape, weight.shape[0])
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        with torch.cuda.device(dy.device):
+            return _FusedProjection._backward(ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
+        need = ctx.needs_input_grad
+        if not any(need[:3]):
+            return None, None, None, dy, None
+        lib = _lib.load()
+        poll_errors()
+        x, weight, z = ctx.saved_tensors
+        M, I, J = ctx.sizes
+        dev = dy.device
+        plan = _lib.product_plan(M, J, I, dev.index)
+        g = _dense(dy)
+
+        def empty(ok, *shape, dtype=torch.bfloat16):
+            return torch.empty(shape, dtype=dtype, device=dev) if ok else None
+
+        dz = empty(z is not None, M, J)
+        dx, dw, db = empty(need[0], M, I), empty(need[1], J, I), empty(need[2], J, dtype=ctx.bias_dtype)
+        part = empty(need[2], plan.dbpart_bytes // 4, dtype=torch.float32)
+        work = empty(plan.backward_work_bytes > 0, plan.backward_work_bytes // 4, dtype=torch.float32)
+        err = _error_word(dev)
+        rc = lib.frnn_b200_product_backward(
+            g.data_ptr(), _ptr(z), _ptr(x), _ptr(weight), _lib.ACTIVATIONS[ctx.activation], _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db),
+            int(ctx.bias_dtype == torch.bfloat16), _ptr(part), M, J, I, _ptr(work), err.data_ptr(), _stream(dev))
+        _track(err, "frnn_b200_product_backward")   # earlier launches of the call have the word, whether a later one was accepted or not
+        _lib.check(rc, "frnn_b200_product_backward")
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def fused_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                     residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``activation(x[..., I] @ weight[J,I].T + bias[J]) + residual[..., J]`` in one kernel, bf16 operands and result, fp32 sums.
+
+    ``activation`` is None, ``"relu"``, ``"silu"`` or ``"gelu_tanh"`` (the tanh form of gelu). x, weight and residual are cast to
+    bf16 where they are of another type, ``bias`` is bf16 or fp32 (others are cast to fp32). Nothing is rounded before the result.
+    Differentiable in all four (once): the gradient at the product, ``dy * activation'(z)``, is rounded to bf16 for the tensor
+    cores; the bias's gradient sums it unrounded. Features that are no multiple of 8 are padded with zeros, at the price of a copy."""
+    tensors = [t for t in (x, weight, bias, residual) if t is not None]
+    if any(t.layout != torch.strided for t in tensors):
+        raise ValueError("inputs must have strided tensor layout")
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"Unknown activation {activation}: None, 'relu', 'silu' or 'gelu_tanh'")
+    if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError("expected x [..., I] and weight [J, I]")
+    J, I = weight.shape
+    if x.numel() < 1 or J < 1:
+        raise ValueError("rows and features must be positive")
+    if bias is not None and tuple(bias.shape) != (J,):
+        raise ValueError("expected bias [J]")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], J):
+        raise ValueError("expected residual [..., J]")
+    if not all(t.is_floating_point() for t in tensors):
+        raise ValueError("inputs must be floating-point tensors")
+    if any(t.device != x.device for t in tensors):
+        raise ValueError("all inputs must be on the same device")
+    if not x.is_cuda:
+        raise RuntimeError("flashrnn_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
+    if torch.cuda.current_device() != x.device.index:
+        with torch.cuda.device(x.device):
+            return _run_product(x, weight, bias, activation, residual)
+    return _run_product(x, weight, bias, activation, residual)
+
+
+def _run_product(x, weight, bias, activation, residual):
+    shape, (J, I) = x.shape, weight.shape
+    x, weight = x.to(torch.bfloat16).reshape(-1, I), weight.to(torch.bfloat16)
+    if residual is not None:
+        residual = residual.to(torch.bfloat16).reshape(-1, J)
+    if bias is not None and bias.dtype != torch.bfloat16:
+        bias = bias.to(torch.float32)
+    pad_i, pad_j = -I % 8, -J % 8
+    if pad_i or pad_j:
+        pad = torch.nn.functional.pad
+        x, weight = pad(x, (0, pad_i)), pad(weight, (0, pad_i, 0, pad_j))
+        bias = None if bias is None else pad(bias, (0, pad_j))
+        residual = None if residual is None else pad(residual, (0, pad_j))
+    x, weight = _dense(x), _dense(weight)
+    bias = None if bias is None else _dense(bias)
+    residual = None if residual is None else _dense(residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        y = _FusedProjection.apply(x, weight, bias, residual, activation)
+    else:
+        y = _product_forward(x, weight, bias, residual, activation, False)[0]
+    return (y[:, :J] if pad_j else y).view(*shape[:-1], J)

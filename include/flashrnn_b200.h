@@ -246,6 +246,31 @@ int frnn_b200_linear_backward(int function, const void* wx, int wx_bf16, const f
                               float* db_part, void* exchange, int B, int T, int N, int D, int wait_limit_ms, int* err, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Matrix product with an epilogue: z = x w^T + bias, y = act(z) + residual. x [rows, inputs], w [outputs, inputs], residual, y,
+ * dy, dz [rows, outputs], dx, dw are bf16; bias and dbias [outputs] fp32 or bf16; inputs % 8 == 0 and outputs % 8 == 0 (else -2),
+ * all pointers 16-byte aligned (else -5). Sums are fp32 in a fixed order. silu: z sigmoid(z); gelu_tanh: the tanh form of gelu. */
+enum { FRNN_ACT_NONE = 0, FRNN_ACT_RELU = 1, FRNN_ACT_SILU = 2, FRNN_ACT_GELU_TANH = 3 };
+
+typedef struct frnn_b200_product_plan {
+  int64_t forward_work_bytes, backward_work_bytes;  /* fp32 partial sums of products with few tiles (0: work may be NULL) */
+  int64_t dbpart_bytes;                             /* scratch for dbias                                                  */
+} frnn_b200_product_plan_t;
+
+/* On the current device (how a product is cut depends on its SM count). */
+int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frnn_b200_product_plan_t* out);
+
+/* bias, residual may be NULL; z: fp16 [rows, outputs], what the backward call takes the activation's slope at, or NULL. y must not
+ * overlap an input. */
+int frnn_b200_product_forward(const void* x, const void* w, const void* bias, int bias_bf16, const void* residual, int activation, void* y,
+                              void* z, int64_t rows, int outputs, int inputs, float* work, int* err, void* stream);
+
+/* dz = dy act'(z) (scratch; z and dz are not used without an activation), dx = dz w, dw = dz^T x, dbias = sum of dz over the rows; dx,
+ * dw, dbias NULL: not wanted. The residual's gradient is dy. */
+int frnn_b200_product_backward(const void* dy, const void* z, const void* x, const void* w, int activation, void* dz, void* dx, void* dw,
+                               void* dbias, int dbias_bf16, float* db_part, int64_t rows, int outputs, int inputs, float* work, int* err,
+                               void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * One WIDE head (N = 1, D a multiple of 256) whose recurrent matrix is split over P GPUs of a node:
  * rank r owns the hidden units [r*Dl, (r+1)*Dl), Dl = D/P (a multiple of 128): the rows R[g, o in slice, :] in the
  * forward pass and the columns R[g, :, p in slice] in the backward pass; the per-step operand (round_bf16(h_t),
