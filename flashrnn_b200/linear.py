@@ -16,20 +16,12 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .functional import _dense, _error_word, _ptr, _stream, _track, poll_errors
 
 # function -> gates of Wx and b
 LINEAR_GATES = {"leaky": 2, "lstm": 4}
-
-
-def _scratch(plan, device):
-    """(exchange buffer, error word) of a launch whose tiles wait for one another, (None, None) of one that has nothing to wait for."""
-    if not plan.exchange_bytes:
-        return None, None
-    return torch.empty(plan.exchange_bytes, dtype=torch.uint8, device=device), _error_word(device)
 
 
 def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Optional[torch.Tensor] = None):
@@ -42,14 +34,16 @@ def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Option
     hidden = torch.empty((B, T, N, D), dtype=wx.dtype, device=dev)
     if last is None:
         last = torch.empty((1, B, 1, N, D), dtype=torch.float32, device=dev)
-    starts = None
-    if keep and plan.starts_bytes:
-        starts = torch.empty(plan.starts_bytes // 4, dtype=torch.float32, device=dev)
-    exchange, err = _scratch(plan, dev)
+    starts = exchange = err = None
+    if plan.exchange_bytes:   # several tiles, which wait for one another
+        exchange, err = torch.empty(plan.exchange_bytes, dtype=torch.uint8, device=dev), _error_word(dev)
+        if keep:
+            starts = torch.empty(plan.starts_bytes // 4, dtype=torch.float32, device=dev)
     rc = lib.frnn_b200_linear_forward(
-        _lib.LINEAR_CELLS[function], wx.data_ptr(), int(wx.dtype == torch.bfloat16), bias.data_ptr(), _ptr(initial), _ptr(lengths),
+        _lib.LINEAR_CELLS[function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
         hidden.data_ptr(), last.data_ptr(), _ptr(starts), _ptr(exchange), B, T, N, D, 0, _ptr(err), _stream(dev))
-    _lib.check(rc, "frnn_b200_linear_forward")
+    if rc:
+        _lib.check(rc, "frnn_b200_linear_forward")
     if err is not None:
         _track(err, "frnn_b200_linear_forward")
     return hidden, last, starts
@@ -65,38 +59,54 @@ class _LinearRecurrence(torch.autograd.Function):
         return hidden, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_hidden, d_last):
-        wx = ctx.saved_tensors[0]
+        _refuse_second_derivative(d_hidden, d_last)
         if d_hidden is None and d_last is None:
-            return (None,) * 5
-        with torch.cuda.device(wx.device):
-            return _LinearRecurrence._backward(ctx, d_hidden, d_last)
+            return None, None, None, None, None
+        wx, bias, initial, lengths, starts = ctx.saved_tensors
+        dev = wx.device
+        if _current_device() != dev.index:
+            with torch.cuda.device(dev):
+                return _LinearRecurrence._backward(ctx, d_hidden, d_last, wx, bias, initial, lengths, starts, dev)
+        return _LinearRecurrence._backward(ctx, d_hidden, d_last, wx, bias, initial, lengths, starts, dev)
 
     @staticmethod
-    def _backward(ctx, d_hidden, d_last):
+    def _backward(ctx, d_hidden, d_last, wx, bias, initial, lengths, starts, dev):
         lib = _lib.load()
         poll_errors()
-        wx, bias, initial, lengths, starts = ctx.saved_tensors
-        B, T, G, N, D = wx.shape
-        dev = wx.device
+        B, T, _, N, D = wx.shape
         plan = _lib.linear_plan(ctx.function, B, T, N, D)
-        d_hidden = torch.zeros((B, T, N, D), dtype=wx.dtype, device=dev) if d_hidden is None else _dense(d_hidden.to(wx.dtype))
+        d_hidden = torch.zeros((B, T, N, D), dtype=wx.dtype, device=dev) if d_hidden is None else _dense(d_hidden)
         if d_last is not None:
-            d_last = d_last.to(torch.float32).contiguous()
+            d_last = d_last.contiguous()
         d_wx, db = torch.empty_like(wx), torch.empty_like(bias)
-        d_initial = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[2] else None
-        db_part = torch.empty(plan.dbpart_bytes // 4, dtype=torch.float32, device=dev) if plan.dbpart_bytes else None
-        exchange, err = _scratch(plan, dev)
+        need = ctx.needs_input_grad
+        d_initial = torch.empty_like(initial) if need[2] else None
+        part = exchange = err = None
+        if plan.dbpart_bytes:   # and the exchange buffer, whose size is 0 where there is nothing to wait for, in one allocation
+            room = (plan.exchange_bytes + 15) // 16 * 16
+            scratch = torch.empty(room + plan.dbpart_bytes, dtype=torch.uint8, device=dev)
+            part = scratch.data_ptr() + room
+            if room:
+                exchange, err = scratch.data_ptr(), _error_word(dev)
         rc = lib.frnn_b200_linear_backward(
-            _lib.LINEAR_CELLS[ctx.function], wx.data_ptr(), int(wx.dtype == torch.bfloat16), bias.data_ptr(), _ptr(initial), _ptr(lengths),
-            _ptr(starts), d_hidden.data_ptr(), _ptr(d_last), d_wx.data_ptr(), db.data_ptr(), _ptr(d_initial), _ptr(db_part),
-            _ptr(exchange), B, T, N, D, 0, _ptr(err), _stream(dev))
+            _lib.LINEAR_CELLS[ctx.function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
+            _ptr(starts), d_hidden.data_ptr(), _ptr(d_last), d_wx.data_ptr(), db.data_ptr(), _ptr(d_initial), part, exchange,
+            B, T, N, D, 0, _ptr(err), _stream(dev))
         if err is not None:
             _track(err, "frnn_b200_linear_backward")   # the scan has the word, whether the sum of db behind it was accepted or not
-        _lib.check(rc, "frnn_b200_linear_backward")
-        need = ctx.needs_input_grad
+        if rc:
+            _lib.check(rc, "frnn_b200_linear_backward")
         return d_wx if need[0] else None, db if need[1] else None, d_initial, None, None
+
+
+def _refuse_second_derivative(*grads) -> None:
+    if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
+        raise RuntimeError("this operator's gradients are not differentiable themselves")
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
 
 
 def flashrnn_linear(Wx: torch.Tensor, b: torch.Tensor, states: Optional[torch.Tensor] = None, function: str = "leaky",
@@ -115,42 +125,50 @@ def flashrnn_linear(Wx: torch.Tensor, b: torch.Tensor, states: Optional[torch.Te
     """
     if function not in LINEAR_GATES:
         raise ValueError(f"Unknown function {function}: flashrnn_linear has {', '.join(LINEAR_GATES)}")
-    tensors = [t for t in (Wx, b, states, lengths, last_out) if t is not None]
-    if any(t.layout != torch.strided for t in tensors):
-        raise ValueError("inputs must have strided tensor layout")
-    if Wx.ndim != 5 or min(Wx.shape) < 1:
-        raise ValueError("expected a nonempty Wx [B,T,G,N,D]")
-    B, T, G, N, D = Wx.shape
-    if G != LINEAR_GATES[function] or tuple(b.shape) != (G, N, D):
-        raise ValueError(f"shape mismatch for {function}: Wx {tuple(Wx.shape)}, b {tuple(b.shape)}")
+    dev, shape = Wx.device, Wx.shape
+    if len(shape) != 5 or Wx.layout != torch.strided or Wx.numel() < 1:
+        raise ValueError("expected a nonempty Wx [B,T,G,N,D] of strided layout")
+    B, T, G, N, D = shape
+    if G != LINEAR_GATES[function] or b.shape != shape[2:]:
+        raise ValueError(f"shape mismatch for {function}: Wx {tuple(shape)}, b {tuple(b.shape)}")
     if Wx.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("Wx must be bfloat16 or float32")
-    if states is not None and tuple(states.shape) != (1, B, 1, N, D):
-        raise ValueError("states must have layout [1,B,1,N,D]")
-    if not b.is_floating_point() or (states is not None and not states.is_floating_point()):
-        raise ValueError("b and states must be floating-point tensors")
-    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
-        raise ValueError("lengths must be an int32 or int64 tensor [B]")
-    if any(t.device != Wx.device for t in tensors):
-        raise ValueError("all inputs must be on the same device")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (Wx, b, states))
+    if b.layout != torch.strided or not b.is_floating_point():
+        raise ValueError("b must be a floating-point tensor of strided layout")
+    same = b.device == dev
+    requires = Wx.requires_grad or b.requires_grad
+    if states is not None:
+        if states.shape != (1, B, 1, N, D):
+            raise ValueError("states must have layout [1,B,1,N,D]")
+        if states.layout != torch.strided or not states.is_floating_point():
+            raise ValueError("states must be a floating-point tensor of strided layout")
+        same = same and states.device == dev
+        requires = requires or states.requires_grad
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.layout != torch.strided or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError("lengths must be an int32 or int64 tensor [B]")
+        same = same and lengths.device == dev
+    requires = requires and torch.is_grad_enabled()
     if last_out is not None:
-        if grad or last_out.requires_grad:
+        if requires or last_out.requires_grad:
             raise ValueError("last_out takes no gradients: call under torch.no_grad()")
-        if tuple(last_out.shape) != (1, B, 1, N, D) or last_out.dtype != torch.float32 or not last_out.is_contiguous():
+        if last_out.shape != (1, B, 1, N, D) or last_out.dtype != torch.float32 or not last_out.is_contiguous():
             raise ValueError("last_out must be a contiguous float32 tensor [1,B,1,N,D]")
+        same = same and last_out.device == dev
+    if not same:
+        raise ValueError("all inputs must be on the same device")
     if not Wx.is_cuda:
         raise RuntimeError("flashrnn_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
-    if torch.cuda.current_device() != Wx.device.index:
-        with torch.cuda.device(Wx.device):
-            return _run(Wx, b, states, function, lengths, last_out, grad)
-    return _run(Wx, b, states, function, lengths, last_out, grad)
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run(Wx, b, states, function, lengths, last_out, requires)
+    return _run(Wx, b, states, function, lengths, last_out, requires)
 
 
 def _run(wx, b, states, function, lengths, last_out, grad):
-    wx, b = _dense(wx), b.to(torch.float32).contiguous()
+    wx, b = _dense(wx), _state(b)
     if states is not None:
-        states = states.to(torch.float32).contiguous()
+        states = _state(states)
     if lengths is not None:
         if lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, wx.shape[1]).to(torch.int32)
@@ -158,14 +176,19 @@ def _run(wx, b, states, function, lengths, last_out, grad):
     if grad:
         return _LinearRecurrence.apply(wx, b, states, lengths, function)
     out = last_out
-    if out is not None and wx.shape[1] > 1:
-        # a longer call may read `states` after other parts of `last` are written: a buffer in between, where they can share memory
-        if states is not None and states.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+    if out is not None and states is not None and states.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+        # a call of several steps may read `states` after other parts of `last` are written, and a step may where the two overlap
+        # without being the same: a buffer in between
+        if wx.shape[1] > 1 or states.data_ptr() != out.data_ptr():
             out = None
-    elif out is not None and states is not None and states.data_ptr() != out.data_ptr() and \
-            states.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
-        out = None
     hidden, last, _ = _forward(wx, b, states, lengths, function, False, out)
-    if last_out is not None and last is not last_out:
+    if last_out is not None and out is None:
         last = last_out.copy_(last)
     return hidden, last
+
+
+def _state(t: torch.Tensor) -> torch.Tensor:
+    """fp32 and contiguous"""
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()

@@ -19,10 +19,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .functional import SIZES, FlashRNNConfig, _dense, _error_word, _ptr, _stream, _track, flashrnn, poll_errors
+from .linear import _current_device, _refuse_second_derivative
 
 
 class _Projection(torch.autograd.Function):
@@ -109,9 +109,10 @@ def _product_forward(x, weight, bias, residual, activation, keep: bool):
     work = torch.empty(plan.forward_work_bytes // 4, dtype=torch.float32, device=dev) if plan.forward_work_bytes else None
     err = _error_word(dev)
     rc = lib.frnn_b200_product_forward(
-        x.data_ptr(), weight.data_ptr(), _ptr(bias), int(bias is not None and bias.dtype == torch.bfloat16), _ptr(residual),
+        x.data_ptr(), weight.data_ptr(), _ptr(bias), bias is not None and bias.dtype == torch.bfloat16, _ptr(residual),
         _lib.ACTIVATIONS[activation], y.data_ptr(), _ptr(z), M, J, I, _ptr(work), err.data_ptr(), _stream(dev))
-    _lib.check(rc, "frnn_b200_product_forward")
+    if rc:
+        _lib.check(rc, "frnn_b200_product_forward")
     _track(err, "frnn_b200_product_forward")
     return y, z
 
@@ -119,45 +120,52 @@ def _product_forward(x, weight, bias, residual, activation, keep: bool):
 class _FusedProjection(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        y, z = _product_forward(x, weight, bias, residual, activation, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None, z)
+        need = ctx.needs_input_grad
+        y, z = _product_forward(x, weight, bias, residual, activation, need[0] or need[1] or need[2])
+        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, z)
         ctx.activation, ctx.sizes = activation, (*x.shape, weight.shape[0])
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        with torch.cuda.device(dy.device):
-            return _FusedProjection._backward(ctx, dy)
+        _refuse_second_derivative(dy)
+        if _current_device() != dy.device.index:
+            with torch.cuda.device(dy.device):
+                return _FusedProjection._backward(ctx, dy, dy.device)
+        return _FusedProjection._backward(ctx, dy, dy.device)
 
     @staticmethod
-    def _backward(ctx, dy):
-        need = ctx.needs_input_grad
-        if not any(need[:3]):
+    def _backward(ctx, dy, dev):
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        if not (need_x or need_w or need_b):
             return None, None, None, dy, None
         lib = _lib.load()
         poll_errors()
         x, weight, z = ctx.saved_tensors
         M, I, J = ctx.sizes
-        dev = dy.device
         plan = _lib.product_plan(M, J, I, dev.index)
         g = _dense(dy)
-
-        def empty(ok, *shape, dtype=torch.bfloat16):
-            return torch.empty(shape, dtype=dtype, device=dev) if ok else None
-
-        dz = empty(z is not None, M, J)
-        dx, dw, db = empty(need[0], M, I), empty(need[1], J, I), empty(need[2], J, dtype=ctx.bias_dtype)
-        part = empty(need[2], plan.dbpart_bytes // 4, dtype=torch.float32)
-        work = empty(plan.backward_work_bytes > 0, plan.backward_work_bytes // 4, dtype=torch.float32)
+        dx = torch.empty((M, I), dtype=torch.bfloat16, device=dev) if need_x else None
+        dw = torch.empty((J, I), dtype=torch.bfloat16, device=dev) if need_w else None
+        db = torch.empty(J, dtype=ctx.bias_dtype, device=dev) if need_b else None
+        # dz, the partial sums of dbias and of the products: one allocation, each part on a 16-byte boundary
+        dz_bytes = 2 * M * J if z is not None else 0
+        part_bytes = (plan.dbpart_bytes + 15) // 16 * 16 if need_b else 0
+        total = dz_bytes + part_bytes + plan.backward_work_bytes
+        at = None
+        if total:
+            scratch = torch.empty(total, dtype=torch.uint8, device=dev)
+            at = scratch.data_ptr()
         err = _error_word(dev)
         rc = lib.frnn_b200_product_backward(
-            g.data_ptr(), _ptr(z), _ptr(x), _ptr(weight), _lib.ACTIVATIONS[ctx.activation], _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db),
-            int(ctx.bias_dtype == torch.bfloat16), _ptr(part), M, J, I, _ptr(work), err.data_ptr(), _stream(dev))
+            g.data_ptr(), _ptr(z), _ptr(x), _ptr(weight), _lib.ACTIVATIONS[ctx.activation], at if dz_bytes else None, _ptr(dx), _ptr(dw),
+            _ptr(db), ctx.bias_dtype == torch.bfloat16, at + dz_bytes if part_bytes else None, M, J, I,
+            at + dz_bytes + part_bytes if plan.backward_work_bytes else None, err.data_ptr(), _stream(dev))
         _track(err, "frnn_b200_product_backward")   # earlier launches of the call have the word, whether a later one was accepted or not
-        _lib.check(rc, "frnn_b200_product_backward")
-        return dx, dw, db, dy if need[3] else None, None
+        if rc:
+            _lib.check(rc, "frnn_b200_product_backward")
+        return dx, dw, db, dy if need_r else None, None
 
 
 def fused_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -168,37 +176,53 @@ def fused_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     bf16 where they are of another type, ``bias`` is bf16 or fp32 (others are cast to fp32). Nothing is rounded before the result.
     Differentiable in all four (once): the gradient at the product, ``dy * activation'(z)``, is rounded to bf16 for the tensor
     cores; the bias's gradient sums it unrounded. Features that are no multiple of 8 are padded with zeros, at the price of a copy."""
-    tensors = [t for t in (x, weight, bias, residual) if t is not None]
-    if any(t.layout != torch.strided for t in tensors):
-        raise ValueError("inputs must have strided tensor layout")
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"Unknown activation {activation}: None, 'relu', 'silu' or 'gelu_tanh'")
-    if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+    dev, shape = x.device, x.shape
+    if len(shape) < 1 or weight.ndim != 2 or weight.shape[1] != shape[-1]:
         raise ValueError("expected x [..., I] and weight [J, I]")
     J, I = weight.shape
     if x.numel() < 1 or J < 1:
         raise ValueError("rows and features must be positive")
-    if bias is not None and tuple(bias.shape) != (J,):
-        raise ValueError("expected bias [J]")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], J):
-        raise ValueError("expected residual [..., J]")
-    if not all(t.is_floating_point() for t in tensors):
+    ok = x.is_floating_point() and weight.is_floating_point()
+    strided = x.layout == torch.strided and weight.layout == torch.strided
+    same = weight.device == dev
+    requires = x.requires_grad or weight.requires_grad
+    if bias is not None:
+        if bias.shape != (J,):
+            raise ValueError("expected bias [J]")
+        ok, strided, same = ok and bias.is_floating_point(), strided and bias.layout == torch.strided, same and bias.device == dev
+        requires = requires or bias.requires_grad
+    if residual is not None:
+        if residual.shape != (*shape[:-1], J):
+            raise ValueError("expected residual [..., J]")
+        ok, same = ok and residual.is_floating_point(), same and residual.device == dev
+        strided = strided and residual.layout == torch.strided
+        requires = requires or residual.requires_grad
+    if not strided:
+        raise ValueError("inputs must have strided tensor layout")
+    if not ok:
         raise ValueError("inputs must be floating-point tensors")
-    if any(t.device != x.device for t in tensors):
+    if not same:
         raise ValueError("all inputs must be on the same device")
     if not x.is_cuda:
         raise RuntimeError("flashrnn_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
-    if torch.cuda.current_device() != x.device.index:
-        with torch.cuda.device(x.device):
-            return _run_product(x, weight, bias, activation, residual)
-    return _run_product(x, weight, bias, activation, residual)
+    requires = requires and torch.is_grad_enabled()
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run_product(x, weight, bias, activation, residual, requires)
+    return _run_product(x, weight, bias, activation, residual, requires)
 
 
-def _run_product(x, weight, bias, activation, residual):
+def _bf16(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16)
+
+
+def _run_product(x, weight, bias, activation, residual, grad: bool):
     shape, (J, I) = x.shape, weight.shape
-    x, weight = x.to(torch.bfloat16).reshape(-1, I), weight.to(torch.bfloat16)
+    x, weight = _bf16(x).reshape(-1, I), _bf16(weight)
     if residual is not None:
-        residual = residual.to(torch.bfloat16).reshape(-1, J)
+        residual = _bf16(residual).reshape(-1, J)
     if bias is not None and bias.dtype != torch.bfloat16:
         bias = bias.to(torch.float32)
     pad_i, pad_j = -I % 8, -J % 8
@@ -208,9 +232,11 @@ def _run_product(x, weight, bias, activation, residual):
         bias = None if bias is None else pad(bias, (0, pad_j))
         residual = None if residual is None else pad(residual, (0, pad_j))
     x, weight = _dense(x), _dense(weight)
-    bias = None if bias is None else _dense(bias)
-    residual = None if residual is None else _dense(residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if bias is not None:
+        bias = _dense(bias)
+    if residual is not None:
+        residual = _dense(residual)
+    if grad:
         y = _FusedProjection.apply(x, weight, bias, residual, activation)
     else:
         y = _product_forward(x, weight, bias, residual, activation, False)[0]

@@ -29,6 +29,7 @@ def test_refusals():
         ("lengths must be", dict(lengths=n[:1])),
         ("lengths must be", dict(lengths=n.float())),
         ("strided", dict(Wx=wx.to_sparse())),
+        ("strided", dict(b=b.to_sparse())),
         ("last_out takes no gradients", dict(Wx=wx.clone().requires_grad_(True), last_out=s.clone())),
         ("last_out must be", dict(last_out=s[:, :1])),
         ("last_out must be", dict(last_out=s.bfloat16())),
