@@ -10,7 +10,7 @@
 // time over e_t = f_t (dc_t + e_{t+1}). The gates' gradients need c_{t-1}: it is recomputed from Wx, which has to be read
 // anyway, and from the state at the start of every tile, which the forward pass keeps (1/128 of a history).
 //
-// One CTA takes a tile of 128 steps x 64 channels of a batch row, read once into registers: a thread has L steps of VEC
+// One CTA takes a tile of 128 (64) steps x 64 channels of a batch row, read once into registers: a thread has L steps of VEC
 // neighbouring channels, scans them, the tile's spans are joined by shuffles and through shared memory, and the second walk over
 // the registers starts from the right state. Tiles of a row are joined through global memory: a tile publishes its (A, H), in
 // groups of 16 tiles every tile composes the maps of those in front of it, in order, with the state at the start of its group,
@@ -24,7 +24,6 @@ namespace frnn {
 
 namespace {
 
-constexpr int kTile = 128;   // steps of a tile
 constexpr int kGroup = 16;   // tiles of a group
 constexpr unsigned long long kDefaultWaitNs = 2000000000ull;
 
@@ -58,8 +57,7 @@ struct Pack {
 #pragma unroll
     for (uint32_t& x : w) x = 0u;
   }
-  __device__ __forceinline__ void load(const void* base, long long elem) {
-    const uint8_t* p = static_cast<const uint8_t*>(base) + elem * (BF16 ? 2 : 4);
+  __device__ __forceinline__ void load(const uint8_t* p) {
     if constexpr (kBytes == 2) {
       w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
     } else if constexpr (kBytes == 4) {
@@ -88,8 +86,7 @@ struct Pack {
       for (int i = 0; i < VEC; i += 2) w[i / 2] = pack_bf16x2(v[i], v[i + 1]);
     }
   }
-  __device__ __forceinline__ void store(void* base, long long elem) const {
-    uint8_t* p = static_cast<uint8_t*>(base) + elem * (BF16 ? 2 : 4);
+  __device__ __forceinline__ void store(uint8_t* p) const {
     if constexpr (kBytes == 2) *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(w[0]);
     else if constexpr (kBytes == 4) *reinterpret_cast<unsigned*>(p) = w[0];
     else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
@@ -97,40 +94,45 @@ struct Pack {
   }
 };
 
+// min that keeps a NaN
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// sigmoid(x) and tanh(y) from a = -log2(e) x and b = -2 log2(e) y with one reciprocal for both: 1 / (1 + 2^a) and
+// (1 - 2^b) / (1 + 2^b). The bounds keep the product of the denominators in range; past them the results are 0 and -1 anyway.
+__device__ __forceinline__ void sigmoid_tanh(float a, float b, float& s, float& t) {
+  const float ea = exp2_fast(min_nan(a, 80.0f)), eb = exp2_fast(min_nan(b, 43.0f)), da = 1.0f + ea, db = 1.0f + eb, r = rcp_fast(da * db);
+  s = db * r;
+  t = (1.0f - eb) * (da * r);
+}
+__device__ __forceinline__ float sigmoid_times_tanh(float a, float b) {
+  const float ea = exp2_fast(min_nan(a, 80.0f)), eb = exp2_fast(min_nan(b, 43.0f));
+  return (1.0f - eb) * rcp_fast((1.0f + ea) * (1.0f + eb));
+}
+
+// Gates arrive as scale(g) (Wx + b): the factor that the exponentials want goes into one fused multiply-add with the bias.
+// kTile: steps of a tile. The LSTM's backward pass holds five values per step and channel: 64 steps leave room for two CTAs.
 template <int CELL> struct LinCell;
 template <> struct LinCell<FRNN_LINEAR_LEAKY> {
-  static constexpr int G = 2;
+  static constexpr int G = 2, kTile = 128;
+  static __device__ __forceinline__ constexpr float scale(int g) { return g == 0 ? kLog2e : 1.0f; }
   static __device__ __forceinline__ void gates(const float* x, float& u, float& v) {
-    u = sigmoid_p(-x[0]);
+    u = rcp_fast(1.0f + exp2_fast(x[0]));
     v = u * x[1];
   }
-  static __device__ __forceinline__ float hidden(const float*, float c) { return c; }
-  // gradient of c through hidden
-  static __device__ __forceinline__ float d_state(const float*, float, float dh) { return dh; }
-  // g: the whole gradient of c_t
-  static __device__ __forceinline__ void d_gates(const float* x, float u, float prev, float, float g, float, float* d) {
-    d[0] = g * (prev - x[1]) * (u * (1.0f - u));
-    d[1] = g * u;
-  }
+  static __device__ __forceinline__ float hidden(float, float c) { return c; }
 };
 template <> struct LinCell<FRNN_LINEAR_LSTM> {
-  static constexpr int G = 4;
+  static constexpr int G = 4, kTile = 64;
+  static __device__ __forceinline__ constexpr float scale(int g) { return g == 1 ? kLog2e : (g == 2 ? -2.0f * kLog2e : -kLog2e); }
   static __device__ __forceinline__ void gates(const float* x, float& u, float& v) {
-    u = sigmoid_p(-x[1]);
-    v = sigmoid_p(x[0]) * tanh_p(x[2]);
+    u = rcp_fast(1.0f + exp2_fast(x[1]));
+    v = sigmoid_times_tanh(x[0], x[2]);
   }
-  static __device__ __forceinline__ float hidden(const float* x, float c) { return sigmoid_p(x[3]) * tanh_p(c); }
-  static __device__ __forceinline__ float d_state(const float* x, float c, float dh) {
-    const float tc = tanh_p(c);
-    return dh * sigmoid_p(x[3]) * (1.0f - tc * tc);
-  }
-  static __device__ __forceinline__ void d_gates(const float* x, float u, float prev, float c, float g, float dh, float* d) {
-    const float i = sigmoid_p(x[0]), z = tanh_p(x[2]), o = sigmoid_p(x[3]), tc = tanh_p(c);
-    d[0] = g * z * (i * (1.0f - i));
-    d[1] = g * prev * (u * (1.0f - u));
-    d[2] = g * i * (1.0f - z * z);
-    d[3] = dh * tc * (o * (1.0f - o));
-  }
+  static __device__ __forceinline__ float hidden(float o, float c) { return sigmoid_times_tanh(o, -2.0f * kLog2e * c); }
 };
 
 // c -> f c + v
@@ -189,21 +191,47 @@ __device__ __forceinline__ void lin_publish(const LinParams& p, const Exchange& 
     st_relaxed_gpu_v2(x.maps + (static_cast<long long>(k) * channels + channel) * 8, xg_clean(__float_as_uint(a)),
                       xg_clean(__float_as_uint(h)));
 }
-// ... every warp fetches that of one tile of the group in front of this one ...
-template <int CW>
-__device__ __forceinline__ void lin_fetch(const LinParams& p, const Exchange& x, int k, int n_channels, float2 (*s_prev)[CW]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp >= k % kGroup) return;
-  const uint8_t* from = x.maps + static_cast<long long>(k / kGroup * kGroup + warp) * CW * 8;
-  for (int c = lane; c < n_channels; c += 32) {
-    uint2 v = make_uint2(kXgFill, kXgFill);
-    lin_poll(p, [&]() {
-      v = ld_relaxed_gpu_v2(from + c * 8);
-      return v.x != kXgFill && v.y != kXgFill;
-    });
-    s_prev[warp][c] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+// ... the warps fetch those of the group's tiles in front of this one, asked for before the tile's own work and again where one had
+// not been there ...
+template <int CW, int NW>
+struct Fetched {
+  static constexpr int kTiles = (kGroup - 1 + NW - 1) / NW, kWords = CW / 32;
+  uint2 map[kTiles][kWords];
+  const uint8_t* from;
+  int n_channels, count;  // count: tiles of the group in front of this one
+  __device__ __forceinline__ void ask(const LinParams& p, const Exchange& x, int k, int channels) {
+    from = x.maps + static_cast<long long>(k / kGroup * kGroup) * CW * 8;
+    n_channels = channels;
+    count = k % kGroup;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        const int q = (threadIdx.x >> 5) + i * NW, c = (threadIdx.x & 31) + 32 * j;
+        if (q < count && c < n_channels) map[i][j] = ld_relaxed_gpu_v2(from + (q * CW + c) * 8);
+      }
+    }
   }
-}
+  __device__ __forceinline__ void put(const LinParams& p, float2 (*s_prev)[CW]) {
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        const int q = (threadIdx.x >> 5) + i * NW, c = (threadIdx.x & 31) + 32 * j;
+        if (q >= count || c >= n_channels) continue;
+        uint2 v = map[i][j];
+        if (v.x == kXgFill || v.y == kXgFill) {
+          const uint8_t* at = from + (q * CW + c) * 8;
+          lin_poll(p, [&]() {
+            v = ld_relaxed_gpu_v2(at);
+            return v.x != kXgFill && v.y != kXgFill;
+          });
+        }
+        s_prev[q][c] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+      }
+    }
+  }
+};
 // ... and they are composed in order with the state at the start of the group, which the last tile of the group before hands out.
 template <int CW>
 __device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x, int k, int channel, const float2 (*s_prev)[CW], float first,
@@ -237,12 +265,24 @@ __device__ __forceinline__ int lin_tile(const LinParams& p, int* shared) {
   return *shared;
 }
 
-// From the maps of the CTA's warps in s_map to the value that each of them starts from, in s_start; warps count backwards in reverse
-// time. `first` [B][ND] (null: zeros) is what the row starts from; done(state, carry, end) is called per channel with its place in
-// [B][ND], what the tile starts from and what it ends with.
-template <int CW, bool REVERSE, typename F>
-__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, const float* first, float2 (*s_map)[CW], float2 (*s_prev)[CW],
-                                         float (*s_start)[CW], F done) {
+// What the CTA's warps share: their maps, the maps of earlier tiles, the values that the warps start from.
+template <int CW, int NW>
+struct Shared {
+  float a[NW][CW], h[NW][CW], start[NW][CW];
+  float2 prev[kGroup - 1][CW];
+};
+
+template <int VEC>
+__device__ __forceinline__ void ld_vec(const float* p, float (&v)[VEC]) { ld_f32_vec<VEC>(p, v); }
+template <int VEC>
+__device__ __forceinline__ void st_vec(float* p, const float (&v)[VEC]) { st_f32_vec<VEC>(p, v); }
+
+// From the maps of the CTA's warps to the value that each of them starts from; warps count backwards in reverse time. `first` [B][ND]
+// (null: zeros) is what the row starts from; done(state, channel, carry, end) is called per channel with its place in [B][ND], what
+// the tile starts from and what it ends with. The maps are in place and a barrier is behind them.
+template <int CW, int NW, bool REVERSE, typename F>
+__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, const float* first, Shared<CW, NW>& s, const Fetched<CW, NW>& got,
+                                         F done) {
   const int nw = blockDim.x >> 5, b = row / p.n_cg, c0 = (row % p.n_cg) * CW, n_channels = min(CW, p.ND - c0);
   const Exchange x(p, row, CW);
   float a[CW / 32], h[CW / 32];
@@ -251,17 +291,17 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, con
     const int c = threadIdx.x + r * blockDim.x;
     a[r] = 1.0f; h[r] = 0.0f;
     if (c >= n_channels) continue;
+#pragma unroll 4
     for (int i = 0; i < nw; ++i) {
       const int w = REVERSE ? nw - 1 - i : i;
-      const float2 m = s_map[w][c];
-      s_map[w][c] = make_float2(a[r], h[r]);
-      h[r] = fmaf(m.x, h[r], m.y);
-      a[r] *= m.x;
+      const float wa = s.a[w][c], wh = s.h[w][c];
+      h[r] = fmaf(wa, h[r], wh);
+      a[r] *= wa;
     }
     if (p.n_tiles > 1) lin_publish(p, x, k, c, CW, a[r], h[r]);
   }
   if (p.n_tiles > 1) {
-    lin_fetch<CW>(p, x, k, n_channels, s_prev);
+    const_cast<Fetched<CW, NW>&>(got).put(p, s.prev);
     __syncthreads();
   }
 #pragma unroll
@@ -270,307 +310,408 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, con
     if (c >= n_channels) continue;
     const long long state = static_cast<long long>(b) * p.ND + c0 + c;
     float carry = first != nullptr && k < kGroup ? __ldg(first + state) : 0.0f;
-    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, c, s_prev, carry, a[r], h[r]);
+    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, c, s.prev, carry, a[r], h[r]);
     done(state, c0 + c, carry, fmaf(a[r], carry, h[r]));
-    for (int w = 0; w < nw; ++w) s_start[w][c] = fmaf(s_map[w][c].x, carry, s_map[w][c].y);
+#pragma unroll 4
+    for (int i = 0; i < nw; ++i) {
+      const int w = REVERSE ? nw - 1 - i : i;
+      s.start[w][c] = carry;
+      carry = fmaf(s.a[w][c], carry, s.h[w][c]);
+    }
   }
   __syncthreads();
 }
 
-template <int CELL, int VEC, int L, int NW, bool BF16>
-__global__ void __launch_bounds__(NW * 32, 2) linear_fwd_kernel(const LinParams p) {
+// This thread's part of a tile.
+template <int VEC, int L, int TILE>
+struct Place {
+  int k, row, b, c0, chl, ch, warp, span, t0, len;
+  bool ok, whole;  // ok: the channels exist; whole: and so do all steps of the warp
+  __device__ __forceinline__ Place(const LinParams& p, int id, bool reverse) {
+    using W = Lanes<VEC>;
+    const int lane = threadIdx.x & 31, rows = p.B * p.n_cg;
+    warp = threadIdx.x >> 5;
+    k = id / rows;
+    row = id - k * rows;
+    if (reverse) k = p.n_tiles - 1 - k;
+    b = row / p.n_cg;
+    c0 = (row - b * p.n_cg) * W::kChannels;
+    span = lane / W::kRow;
+    chl = (lane % W::kRow) * VEC;
+    ch = c0 + chl;
+    t0 = k * TILE + (warp * W::kSpans + span) * L;
+    ok = ch < p.ND;
+    len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
+    whole = k * TILE + (warp + 1) * W::kSpans * L <= len && c0 + W::kChannels <= p.ND;
+  }
+  __device__ __forceinline__ bool valid(int l) const { return ok && t0 + l < len; }
+};
+
+// The maps of the warp's spans, one to a lane, become those of what lies in front of each (behind, in reverse time); that of the whole
+// warp goes to (a, h) in shared memory.
+template <int VEC, bool REVERSE>
+__device__ __forceinline__ void join_spans(int span, float (&A)[VEC], float (&H)[VEC], float* a, float* h) {
+  using W = Lanes<VEC>;
+  auto from = [&](float v, int o) {
+    return REVERSE ? __shfl_down_sync(0xffffffffu, v, o * W::kRow) : __shfl_up_sync(0xffffffffu, v, o * W::kRow);
+  };
+  const int at = REVERSE ? W::kSpans - 1 - span : span;  // place in the order of the scan
+#pragma unroll
+  for (int o = 1; o < W::kSpans; o *= 2) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float pa = from(A[i], o), ph = from(H[i], o);
+      if (at >= o) {
+        H[i] = fmaf(A[i], ph, H[i]);
+        A[i] *= pa;
+      }
+    }
+  }
+  if (at == W::kSpans - 1) {
+    st_vec<VEC>(a, A);
+    st_vec<VEC>(h, H);
+  }
+  if constexpr (W::kSpans > 1) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      A[i] = from(A[i], 1);
+      H[i] = from(H[i], 1);
+    }
+  }
+  if (at == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
+  }
+}
+
+template <int CELL, int VEC>
+__device__ __forceinline__ void load_bias(const LinParams& p, bool ok, int ch, float (&bias)[LinCell<CELL>::G][VEC]) {
+#pragma unroll
+  for (int g = 0; g < LinCell<CELL>::G; ++g) {
+    if (ok) {
+      ld_vec<VEC>(p.bias + static_cast<long long>(g) * p.ND + ch, bias[g]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) bias[g][i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) bias[g][i] *= LinCell<CELL>::scale(g);
+  }
+}
+
+template <int CELL, int VEC, int L, int NW, int MIN_CTAS, bool BF16>
+__global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const LinParams p) {
   using W = Lanes<VEC>;
   using Cell = LinCell<CELL>;
   constexpr int G = Cell::G, CW = W::kChannels;
-  static_assert(NW * W::kSpans * L == kTile && NW >= kGroup - 1, "a full CTA covers a tile");
-  __shared__ float2 s_map[NW][CW], s_prev[kGroup - 1][CW];
-  __shared__ float s_start[NW][CW];
+  static_assert(NW * W::kSpans * L == Cell::kTile, "a full CTA covers a tile");
+  __shared__ __align__(16) Shared<CW, NW> s;
   __shared__ int s_tile;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int id = lin_tile(p, &s_tile);
-  const int rows = p.B * p.n_cg, k = id / rows, row = id % rows, b = row / p.n_cg, c0 = (row % p.n_cg) * CW;
-  const int span = lane / W::kRow, chl = (lane % W::kRow) * VEC, ch = c0 + chl;
-  const int t0 = k * kTile + (warp * W::kSpans + span) * L;
-  const bool ok = ch < p.ND;
-  const int len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
-  const int len_here = ok ? len : 0;  // channels past the last are no steps at all
+  const Place<VEC, L, Cell::kTile> at(p, id, false);
 
+  const size_t es = BF16 ? 2 : 4, gate = static_cast<size_t>(p.ND) * es;
+  const uint8_t* from = static_cast<const uint8_t*>(p.wx) + ((static_cast<size_t>(at.b) * p.T + at.t0) * G * p.ND + at.ch) * es;
   Pack<VEC, BF16> raw[L][G];
+  if (at.whole) {
 #pragma unroll
-  for (int l = 0; l < L; ++l) {
-    const long long at = ((static_cast<long long>(b) * p.T + t0 + l) * G) * p.ND + ch;
+    for (int l = 0; l < L; ++l)
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (t0 + l < len_here) raw[l][g].load(p.wx, at + static_cast<long long>(g) * p.ND);
-      else raw[l][g].clear();
-    }
+      for (int g = 0; g < G; ++g) raw[l][g].load(from + (l * G + g) * gate);
+  } else {
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (at.valid(l)) raw[l][g].load(from + (l * G + g) * gate);
+        else raw[l][g].clear();
+      }
   }
+  Fetched<CW, NW> got;
+  if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), at.k, min(CW, p.ND - at.c0));
   float bias[G][VEC];
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) bias[g][i] = ok ? __ldg(p.bias + static_cast<long long>(g) * p.ND + ch + i) : 0.0f;
+  load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  float u[L][VEC], v[L][VEC], A[VEC], H[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
+  // the maps of this thread's steps up to each of them
+  float A[L][VEC], H[L][VEC], a[VEC], h[VEC];
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    const bool valid = t0 + l < len_here;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       float x[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = raw[l][g].get(i) + bias[g][i];
-      Cell::gates(x, u[l][i], v[l][i]);
-      if (!valid) u[l][i] = v[l][i] = 0.0f;  // a step behind the end of a sequence leaves its state alone
-      H[i] = lin_step(u[l][i], v[l][i], H[i]);
-      A[i] = fmaf(-u[l][i], A[i], A[i]);
+      for (int g = 0; g < G; ++g) x[g] = fmaf(raw[l][g].get(i), Cell::scale(g), bias[g][i]);
+      Cell::gates(x, A[l][i], H[l][i]);  // u and v
     }
   }
-  // spans of the warp in front of this one
+  if (!at.whole) {  // a step behind the end of a sequence leaves its state alone
 #pragma unroll
-  for (int o = 1; o < W::kSpans; o *= 2) {
+    for (int l = 0; l < L; ++l)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float pa = __shfl_up_sync(0xffffffffu, A[i], o * W::kRow), ph = __shfl_up_sync(0xffffffffu, H[i], o * W::kRow);
-      if (span >= o) {
-        H[i] = fmaf(A[i], ph, H[i]);
-        A[i] *= pa;
-      }
-    }
+      for (int i = 0; i < VEC; ++i)
+        if (!at.valid(l)) A[l][i] = H[l][i] = 0.0f;
   }
-  if (span == W::kSpans - 1) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s_map[warp][chl + i] = make_float2(A[i], H[i]);
-  }
-  if constexpr (W::kSpans > 1) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      A[i] = __shfl_up_sync(0xffffffffu, A[i], W::kRow);
-      H[i] = __shfl_up_sync(0xffffffffu, H[i], W::kRow);
-    }
-  }
-  if (span == 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
-  }
-  __syncthreads();
-  lin_join<CW, false>(p, row, k, p.initial, s_map, s_prev, s_start, [&](long long state, int channel, float carry, float end) {
-    if (p.starts != nullptr && k > 0) p.starts[(static_cast<long long>(b) * (p.n_tiles - 1) + k - 1) * p.ND + channel] = carry;
-    if (k == p.n_tiles - 1) p.last[state] = end;
-  });
-  if (!ok) return;
-  float c[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = fmaf(A[i], s_start[warp][chl + i], H[i]);
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    if (t0 + l < p.T) {
-      float out[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float x[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) x[g] = raw[l][g].get(i) + bias[g][i];
-        c[i] = lin_step(u[l][i], v[l][i], c[i]);
-        out[i] = t0 + l < len ? Cell::hidden(x, c[i]) : 0.0f;
+    for (int i = 0; i < VEC; ++i) {
+      const float u = A[l][i], v = H[l][i];
+      if (l == 0) {
+        A[0][i] = 1.0f - u;
+      } else {
+        H[l][i] = lin_step(u, v, H[l - 1][i]);
+        A[l][i] = fmaf(-u, A[l - 1][i], A[l - 1][i]);
       }
-      Pack<VEC, BF16> w;
-      w.set(out);
-      w.store(p.hidden, (static_cast<long long>(b) * p.T + t0 + l) * p.ND + ch);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) { a[i] = A[L - 1][i]; h[i] = H[L - 1][i]; }
+  join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
+  __syncthreads();
+  lin_join<CW, NW, false>(p, at.row, at.k, p.initial, s, got, [&](long long state, int channel, float carry, float end) {
+    if (p.starts != nullptr && at.k > 0) p.starts[(static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + channel] = carry;
+    if (at.k == p.n_tiles - 1) p.last[state] = end;
+  });
+  if (!at.ok) return;
+  float c[VEC];
+  ld_vec<VEC>(&s.start[at.warp][at.chl], c);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) c[i] = fmaf(a[i], c[i], h[i]);
+  const size_t step = static_cast<size_t>(p.ND) * es;
+  uint8_t* to = static_cast<uint8_t*>(p.hidden) + ((static_cast<size_t>(at.b) * p.T + at.t0) * p.ND + at.ch) * es;
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    float out[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float o = G == 4 ? fmaf(raw[l][G - 1].get(i), Cell::scale(G - 1), bias[G - 1][i]) : 0.0f;
+      out[i] = Cell::hidden(o, fmaf(A[l][i], c[i], H[l][i]));
+    }
+    if (!at.whole) {
+      if (at.t0 + l >= p.T) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[i] = at.valid(l) ? out[i] : 0.0f;
+    }
+    Pack<VEC, BF16> w;
+    w.set(out);
+    w.store(to + l * step);
   }
 }
 
-template <int CELL, int VEC, int L, int NW, bool BF16>
-__global__ void __launch_bounds__(NW * 32, CELL == FRNN_LINEAR_LEAKY ? 2 : 1) linear_bwd_kernel(const LinParams p) {
+template <int CELL, int VEC, int L, int NW, int MIN_CTAS, bool BF16>
+__global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const LinParams p) {
   using W = Lanes<VEC>;
   using Cell = LinCell<CELL>;
   constexpr int G = Cell::G, CW = W::kChannels;
-  static_assert(NW * W::kSpans * L == kTile && NW >= kGroup - 1, "a full CTA covers a tile");
-  // maps and starts of the recomputed states and of the gradients in reverse time; then the parts of db
-  __shared__ float2 s_map[2][NW][CW], s_prev[kGroup - 1][CW];
-  __shared__ float s_start[2][NW][CW];
+  static_assert(NW * W::kSpans * L == Cell::kTile, "a full CTA covers a tile");
+  __shared__ __align__(16) Shared<CW, NW> s;
+  __shared__ __align__(16) float s_db[NW][G][CW];  // first the maps of the recomputed states and what their warps start from
   __shared__ int s_tile;
-  static_assert(sizeof(s_map) >= sizeof(float) * NW * G * CW, "parts of db take the room of the maps");
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nw = blockDim.x >> 5;
+  static_assert(G >= 2, "room for the maps");
+  float(*f_a)[CW] = reinterpret_cast<float(*)[CW]>(&s_db[0][0][0]);  // [NW][CW]
+  float(*f_h)[CW] = f_a + NW;
+  const int tid = threadIdx.x, nw = blockDim.x >> 5;
   const int id = lin_tile(p, &s_tile);
-  const int rows = p.B * p.n_cg, kr = id / rows, k = p.n_tiles - 1 - kr;  // kr: in the order of the scan
-  const int row = id % rows, b = row / p.n_cg, c0 = (row % p.n_cg) * CW;
-  const int span = lane / W::kRow, chl = (lane % W::kRow) * VEC, ch = c0 + chl;
-  const int t0 = k * kTile + (warp * W::kSpans + span) * L;
-  const bool ok = ch < p.ND;
-  const int len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
-  const int len_here = ok ? len : 0;
+  const Place<VEC, L, Cell::kTile> at(p, id, true);
+  const int kr = p.n_tiles - 1 - at.k;  // in the order of the scan
 
+  const size_t es = BF16 ? 2 : 4, row_bytes = static_cast<size_t>(p.ND) * es, first = static_cast<size_t>(at.b) * p.T + at.t0;
+  const uint8_t* from = static_cast<const uint8_t*>(p.wx) + (first * G * p.ND + at.ch) * es;
+  const uint8_t* from_dh = static_cast<const uint8_t*>(p.d_hidden) + (first * p.ND + at.ch) * es;
+  uint8_t* to = static_cast<uint8_t*>(p.d_wx) + (first * G * p.ND + at.ch) * es;
   Pack<VEC, BF16> raw[L][G], raw_dh[L];
+  if (at.whole) {
 #pragma unroll
-  for (int l = 0; l < L; ++l) {
-    const long long step = static_cast<long long>(b) * p.T + t0 + l;
+    for (int l = 0; l < L; ++l) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (t0 + l < len_here) raw[l][g].load(p.wx, (step * G + g) * p.ND + ch);
-      else raw[l][g].clear();
+      for (int g = 0; g < G; ++g) raw[l][g].load(from + (l * G + g) * row_bytes);
+      raw_dh[l].load(from_dh + l * row_bytes);
     }
-    if (t0 + l < len_here) raw_dh[l].load(p.d_hidden, step * p.ND + ch);
-    else raw_dh[l].clear();
-  }
-  float bias[G][VEC];
+  } else {
 #pragma unroll
-  for (int g = 0; g < G; ++g)
+    for (int l = 0; l < L; ++l) {
+      if (at.valid(l)) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) bias[g][i] = ok ? __ldg(p.bias + static_cast<long long>(g) * p.ND + ch + i) : 0.0f;
-
-  // the states, as in the forward kernel
-  float u[L][VEC], prev[L][VEC], A[VEC], H[VEC], total[VEC];
+        for (int g = 0; g < G; ++g) raw[l][g].load(from + (l * G + g) * row_bytes);
+        raw_dh[l].load(from_dh + l * row_bytes);
+      } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
-#pragma unroll
-  for (int l = 0; l < L; ++l) {
-    const bool valid = t0 + l < len_here;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float x[G], v;
-#pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = raw[l][g].get(i) + bias[g][i];
-      Cell::gates(x, u[l][i], v);
-      if (!valid) u[l][i] = v = 0.0f;
-      prev[l][i] = v;  // until the states are known
-      H[i] = lin_step(u[l][i], v, H[i]);
-      A[i] = fmaf(-u[l][i], A[i], A[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) total[i] = A[i];  // the decay over this thread's steps
-#pragma unroll
-  for (int o = 1; o < W::kSpans; o *= 2) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float pa = __shfl_up_sync(0xffffffffu, A[i], o * W::kRow), ph = __shfl_up_sync(0xffffffffu, H[i], o * W::kRow);
-      if (span >= o) {
-        H[i] = fmaf(A[i], ph, H[i]);
-        A[i] *= pa;
+        for (int g = 0; g < G; ++g) raw[l][g].clear();
+        raw_dh[l].clear();
       }
     }
   }
-  if (span == W::kSpans - 1) {
+  Fetched<CW, NW> got;
+  if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), kr, min(CW, p.ND - at.c0));
+  // the state in front of the tile, channels as in lin_join
+  float before[CW / 32];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s_map[0][warp][chl + i] = make_float2(A[i], H[i]);
+  for (int r = 0; r < CW / 32; ++r) {
+    const int c = tid + r * blockDim.x;
+    before[r] = 0.0f;
+    if (c >= min(CW, p.ND - at.c0)) continue;
+    if (at.k > 0) before[r] = __ldg(p.starts + (static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + at.c0 + c);
+    else if (p.initial != nullptr) before[r] = __ldg(p.initial + static_cast<long long>(at.b) * p.ND + at.c0 + c);
   }
-  if constexpr (W::kSpans > 1) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      A[i] = __shfl_up_sync(0xffffffffu, A[i], W::kRow);
-      H[i] = __shfl_up_sync(0xffffffffu, H[i], W::kRow);
-    }
-  }
-  if (span == 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
-  }
-  __syncthreads();
-  for (int c = tid; c < CW; c += blockDim.x) {
-    if (c0 + c >= p.ND) continue;
-    float h = 0.0f;
-    if (k > 0) h = __ldg(p.starts + (static_cast<long long>(b) * (p.n_tiles - 1) + k - 1) * p.ND + c0 + c);
-    else if (p.initial != nullptr) h = __ldg(p.initial + static_cast<long long>(b) * p.ND + c0 + c);
-    for (int w = 0; w < nw; ++w) {
-      s_start[0][w][c] = h;
-      h = fmaf(s_map[0][w][c].x, h, s_map[0][w][c].y);
-    }
-  }
-  __syncthreads();
-  float c[VEC], dc[L][VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = ok ? fmaf(A[i], s_start[0][warp][chl + i], H[i]) : 0.0f;
+  float bias[G][VEC];
+  load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
+
+  // u; the state in front of each step; the LSTM's i and z
+  float u[L][VEC], prev[L][VEC], si[G == 4 ? L : 1][VEC], tz[G == 4 ? L : 1][VEC], A[VEC], H[VEC];
 #pragma unroll
   for (int l = 0; l < L; ++l) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       float x[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = raw[l][g].get(i) + bias[g][i];
-      const float v = prev[l][i];
-      prev[l][i] = c[i];
-      c[i] = lin_step(u[l][i], v, c[i]);
-      dc[l][i] = t0 + l < len_here ? Cell::d_state(x, c[i], raw_dh[l].get(i)) : 0.0f;
-    }
-  }
-  // the gradients that leave every span towards earlier steps
-  float E[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) { A[i] = total[i]; E[i] = 0.0f; }
-#pragma unroll
-  for (int l = L - 1; l >= 0; --l) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float g = dc[l][i] + E[i];
-      E[i] = fmaf(-u[l][i], g, g);
-    }
-  }
-#pragma unroll
-  for (int o = 1; o < W::kSpans; o *= 2) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float pa = __shfl_down_sync(0xffffffffu, A[i], o * W::kRow), pe = __shfl_down_sync(0xffffffffu, E[i], o * W::kRow);
-      if (span + o < W::kSpans) {
-        E[i] = fmaf(A[i], pe, E[i]);
-        A[i] *= pa;
+      for (int g = 0; g < G; ++g) x[g] = fmaf(raw[l][g].get(i), Cell::scale(g), bias[g][i]);
+      if constexpr (G == 4) {
+        u[l][i] = rcp_fast(1.0f + exp2_fast(x[1]));
+        sigmoid_tanh(x[0], x[2], si[l][i], tz[l][i]);
+        prev[l][i] = si[l][i] * tz[l][i];
+      } else {
+        Cell::gates(x, u[l][i], prev[l][i]);  // v, until the states are known
       }
     }
   }
-  if (span == 0) {
+  if (!at.whole) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s_map[1][warp][chl + i] = make_float2(A[i], E[i]);
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (!at.valid(l)) u[l][i] = prev[l][i] = 0.0f;
   }
-  if constexpr (W::kSpans > 1) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      A[i] = __shfl_down_sync(0xffffffffu, A[i], W::kRow);
-      E[i] = __shfl_down_sync(0xffffffffu, E[i], W::kRow);
+  for (int i = 0; i < VEC; ++i) {
+    A[i] = 1.0f - u[0][i];
+    H[i] = prev[0][i];
+#pragma unroll
+    for (int l = 1; l < L; ++l) {
+      H[i] = lin_step(u[l][i], prev[l][i], H[i]);
+      A[i] = fmaf(-u[l][i], A[i], A[i]);
     }
   }
-  if (span == W::kSpans - 1) {
+  join_spans<VEC, false>(at.span, A, H, &f_a[at.warp][at.chl], &f_h[at.warp][at.chl]);
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; E[i] = 0.0f; }
+  for (int r = 0; r < CW / 32; ++r) {
+    const int c = tid + r * blockDim.x;
+    if (c >= min(CW, p.ND - at.c0)) continue;
+    float v = before[r];
+#pragma unroll 4
+    for (int w = 0; w < nw; ++w) {
+      s.start[w][c] = v;
+      v = fmaf(f_a[w][c], v, f_h[w][c]);
+    }
   }
   __syncthreads();
-  lin_join<CW, true>(p, row, kr, p.d_last, s_map[1], s_prev, s_start[1], [&](long long state, int, float, float end) {
-    if (k == 0 && p.d_initial != nullptr) p.d_initial[state] = end;
-  });
-  float db[G][VEC];
+  float c[VEC], db[G][VEC];
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) db[g][i] = 0.0f;
+  if (at.ok) {
+    ld_vec<VEC>(&s.start[at.warp][at.chl], c);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) E[i] = ok ? fmaf(A[i], s_start[1][warp][chl + i], E[i]) : 0.0f;
+    for (int i = 0; i < VEC; ++i) c[i] = 0.0f;
+  }
 #pragma unroll
-  for (int l = L - 1; l >= 0; --l) {
-    const bool valid = t0 + l < len_here;
-    float d[G][VEC];
+  for (int i = 0; i < VEC; ++i) c[i] = fmaf(A[i], c[i], H[i]);
+  // the gradient of each state through its hidden state; the output gate's is done with
+  float dc[G == 4 ? L : 1][VEC];
+  auto d_state = [&](int l, int i) {
+    if constexpr (G == 4) return dc[l][i];
+    else return raw_dh[l].get(i);
+  };
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    float d_o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      float x[G], dg[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = raw[l][g].get(i) + bias[g][i];
-      const float g_c = dc[l][i] + E[i];
-      E[i] = fmaf(-u[l][i], g_c, g_c);
-      Cell::d_gates(x, u[l][i], prev[l][i], c[i], g_c, raw_dh[l].get(i), dg);
-      c[i] = prev[l][i];
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        d[g][i] = valid ? dg[g] : 0.0f;
-        db[g][i] += d[g][i];
+      const float v = prev[l][i];
+      prev[l][i] = c[i];
+      c[i] = lin_step(u[l][i], v, c[i]);
+      if constexpr (G == 4) {
+        float o, tc;
+        sigmoid_tanh(fmaf(raw[l][3].get(i), Cell::scale(3), bias[3][i]), -2.0f * kLog2e * c[i], o, tc);
+        const float dh_o = raw_dh[l].get(i) * o;
+        dc[l][i] = dh_o * fmaf(-tc, tc, 1.0f);
+        d_o[i] = dh_o * tc * (1.0f - o);
+        if (!at.whole && !at.valid(l)) dc[l][i] = d_o[i] = 0.0f;
+        db[3][i] += d_o[i];
       }
     }
-    if (ok && t0 + l < p.T) {
+    if constexpr (G == 4) {
+      if (at.whole || (at.ok && at.t0 + l < p.T)) {
+        Pack<VEC, BF16> w;
+        w.set(d_o);
+        w.store(to + (l * G + 3) * row_bytes);
+      }
+    }
+  }
+  // what leaves this thread's steps towards earlier ones
+  float E[VEC];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
+  for (int i = 0; i < VEC; ++i) {
+    const float g0 = d_state(L - 1, i);
+    E[i] = fmaf(-u[L - 1][i], g0, g0);
+    A[i] = 1.0f - u[L - 1][i];
+#pragma unroll
+    for (int l = L - 2; l >= 0; --l) {
+      const float g = d_state(l, i) + E[i];
+      E[i] = fmaf(-u[l][i], g, g);
+      A[i] = fmaf(-u[l][i], A[i], A[i]);
+    }
+  }
+  join_spans<VEC, true>(at.span, A, E, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
+  __syncthreads();
+  lin_join<CW, NW, true>(p, at.row, kr, p.d_last, s, got, [&](long long state, int, float, float end) {
+    if (at.k == 0 && p.d_initial != nullptr) p.d_initial[state] = end;
+  });
+  float e[VEC];
+  if (at.ok) {
+    ld_vec<VEC>(&s.start[at.warp][at.chl], e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) E[i] = fmaf(A[i], e[i], E[i]);
+#pragma unroll
+  for (int l = L - 1; l >= 0; --l) {
+    constexpr int kHere = G == 4 ? 3 : G;  // gates whose gradients are stored here
+    float d[kHere][VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float g = d_state(l, i) + E[i], q = fmaf(-u[l][i], u[l][i], u[l][i]);  // u (1 - u)
+      E[i] = fmaf(-u[l][i], g, g);
+      if constexpr (G == 4) {
+        const float gi = g * si[l][i];
+        d[0][i] = gi * tz[l][i] * (1.0f - si[l][i]);
+        d[1][i] = g * prev[l][i] * q;
+        d[2][i] = gi * fmaf(-tz[l][i], tz[l][i], 1.0f);
+      } else {
+        d[0][i] = g * (prev[l][i] - (raw[l][1].get(i) + bias[1][i])) * q;
+        d[1][i] = g * u[l][i];
+      }
+    }
+    if (!at.whole) {
+#pragma unroll
+      for (int g = 0; g < kHere; ++g)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d[g][i] = at.valid(l) ? d[g][i] : 0.0f;
+    }
+#pragma unroll
+    for (int g = 0; g < kHere; ++g)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) db[g][i] += d[g][i];
+    if (at.whole || (at.ok && at.t0 + l < p.T)) {
+#pragma unroll
+      for (int g = 0; g < kHere; ++g) {
         Pack<VEC, BF16> w;
         w.set(d[g]);
-        w.store(p.d_wx, ((static_cast<long long>(b) * p.T + t0 + l) * G + g) * p.ND + ch);
+        w.store(to + (l * G + g) * row_bytes);
       }
     }
   }
@@ -581,20 +722,17 @@ __global__ void __launch_bounds__(NW * 32, CELL == FRNN_LINEAR_LEAKY ? 2 : 1) li
 #pragma unroll
       for (int i = 0; i < VEC; ++i) db[g][i] += __shfl_xor_sync(0xffffffffu, db[g][i], o);
   }
-  float* s_db = reinterpret_cast<float*>(&s_map[0][0][0]);  // [nw][G][CW]; the maps were last read in front of the last barrier
-  if (span == 0) {
+  if (at.span == 0) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s_db[(warp * G + g) * CW + chl + i] = db[g][i];
+    for (int g = 0; g < G; ++g) st_vec<VEC>(&s_db[at.warp][g][at.chl], db[g]);
   }
   __syncthreads();
   for (int j = tid; j < G * CW; j += blockDim.x) {
     const int g = j / CW, cc = j % CW;
-    if (c0 + cc >= p.ND) continue;
+    if (at.c0 + cc >= p.ND) continue;
     float sum = 0.0f;
-    for (int w = 0; w < nw; ++w) sum += s_db[(w * G + g) * CW + cc];
-    p.db_part[((static_cast<long long>(b) * p.n_tiles + k) * G + g) * p.ND + c0 + cc] = sum;
+    for (int w = 0; w < nw; ++w) sum += s_db[w][g][cc];
+    p.db_part[((static_cast<long long>(at.b) * p.n_tiles + at.k) * G + g) * p.ND + at.c0 + cc] = sum;
   }
 }
 
@@ -616,21 +754,25 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
 int lin_vec(int ND) { return ND % 4 == 0 ? 4 : 1; }
 int lin_channels(int ND) { return lin_vec(ND) == 1 ? 32 : 64; }
 
-template <int CELL, int VEC, int L, int NW, bool BF16>
-int launch_one(LinParams p, bool backward, cudaStream_t s) {
+template <int CELL, int VEC, int LF, int LB, bool BF16>
+int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
+  constexpr int kSpans = Lanes<VEC>::kSpans, kTile = LinCell<CELL>::kTile, kNWF = kTile / (kSpans * LF), kNWB = kTile / (kSpans * LB);
   const long long tiles = static_cast<long long>(p.B) * p.n_cg * p.n_tiles;
   if (tiles > 0x7fffffffLL) return -2;
-  int warps = NW;
-  if (p.n_tiles == 1) warps = (p.T + Lanes<VEC>::kSpans * L - 1) / (Lanes<VEC>::kSpans * L);
-  if (!backward) linear_fwd_kernel<CELL, VEC, L, NW, BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
-  else linear_bwd_kernel<CELL, VEC, L, NW, BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
+  const int l = backward ? LB : LF;
+  int warps = backward ? kNWB : kNWF;
+  if (p.n_tiles == 1) warps = (p.T + kSpans * l - 1) / (kSpans * l);
+  if (!backward) linear_fwd_kernel<CELL, VEC, LF, kNWF, 512 / (kNWF * 32), BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
+  else linear_bwd_kernel<CELL, VEC, LB, kNWB, 512 / (kNWB * 32), BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
+// L, the steps of a thread: 32 values of a thread of the leaky cell, 32 and 16 of the LSTM's.
 template <int CELL, bool BF16>
 int launch_vec(const LinParams& p, bool backward, cudaStream_t s) {
-  if (lin_vec(p.ND) == 4) return launch_one<CELL, 4, 4, 16, BF16>(p, backward, s);
-  return launch_one<CELL, 1, 8, 16, BF16>(p, backward, s);
+  constexpr bool kLstm = CELL == FRNN_LINEAR_LSTM;
+  if (lin_vec(p.ND) == 4) return launch_one<CELL, 4, 8, kLstm ? 4 : 8, BF16>(p, backward, s);
+  return launch_one<CELL, 1, 16, kLstm ? 8 : 16, BF16>(p, backward, s);
 }
 
 int launch(int function, int wx_bf16, const LinParams& p, bool backward, cudaStream_t s) {
@@ -666,11 +808,12 @@ extern "C" int frnn_b200_linear_plan(int function, int B, int T, int N, int D, f
   const int gates = function == FRNN_LINEAR_LEAKY ? 2 : 4;
   if (nd * gates > 0x7fffffffLL) return -2;
   const int channels = lin_channels(static_cast<int>(nd));
-  const long long blocks = B * ((nd + channels - 1) / channels), tiles = (static_cast<long long>(T) + kTile - 1) / kTile;
+  const int steps = function == FRNN_LINEAR_LEAKY ? LinCell<FRNN_LINEAR_LEAKY>::kTile : LinCell<FRNN_LINEAR_LSTM>::kTile;
+  const long long blocks = B * ((nd + channels - 1) / channels), tiles = (static_cast<long long>(T) + steps - 1) / steps;
   if (blocks * tiles > 0x7fffffffLL) return -2;
   *out = {};
   out->gates = gates;
-  out->tile_steps = kTile;
+  out->tile_steps = steps;
   out->tile_channels = channels;
   out->tiles = static_cast<int>(tiles);
   if (tiles > 1) {

@@ -25,10 +25,14 @@ namespace {
 
 constexpr int kThreads = 320;    // warps 0-7 epilogue, 8 TMA, 9 MMA
 constexpr int kEpiWarps = 8;
-constexpr int kStages = 4;
 constexpr int kKC = 64;          // k's per stage: 128 bytes of bf16, one swizzle row
-constexpr int kBufBytes = 4096;  // staging: 32 rows x 128 bytes
-constexpr int kSmem = kStages * 32768 + kEpiWarps * 3 * kBufBytes + 1024;
+constexpr int kBufBytes = 4096;  // staging of a warp: two buffers of 32 rows x 128 bytes
+// Stages of the ring: as many as fit beside the staging buffers. B along N comes in boxes of 64 columns, whole ones.
+__host__ __device__ constexpr int stage_bytes_of(int np, bool b_mn) { return 16384 + (b_mn ? (np / 2 + 63) / 64 * 8192 : np / 2 * 128); }
+__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (227 * 1024 - 2048 - kEpiWarps * 2 * kBufBytes) / stage_bytes_of(np, b_mn); }
+__host__ __device__ constexpr int smem_of(int np, bool b_mn) {
+  return stages_of(np, b_mn) * stage_bytes_of(np, b_mn) + kEpiWarps * 2 * kBufBytes + 1024;
+}
 constexpr uint64_t kLimit = 2000000000ull;
 
 struct ProductParams {
@@ -100,21 +104,47 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, const uint32_t (&v)[4])
 }
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// Two fp16 values; what is past their range becomes the largest one, a NaN stays one.
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  a = fabsf(a) > 65504.0f ? copysignf(65504.0f, a) : a;  // a NaN stays one
-  b = fabsf(b) > 65504.0f ? copysignf(65504.0f, b) : b;
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+// (a, b) <- (a, b) * (c, d) + (e, f)
+__device__ __forceinline__ void fma2(float& a, float& b, float c, float d, float e, float f) {
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n mov.b64 z, {%4, %5};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b) : "f"(c), "f"(d), "f"(e), "f"(f));
 }
 
-// silu and the tanh form of gelu are both z sigmoid(w(z)): z and sqrt(8 / pi) (z + 0.044715 z^3).
-constexpr float kGelu = 1.5957691216057308f, kGeluCube = 0.044715f;
+// silu and the tanh form of gelu are both z sigmoid(w(z)): w = z and sqrt(8 / pi) (z + 0.044715 z^3).
+constexpr float kGelu = 1.5957691216057308f, kGeluCube = 0.044715f, kLog2e = 1.4426950408889634f;
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (ACT == FRNN_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if constexpr (ACT == FRNN_ACT_SILU) return z * sigmoid_p(z);
-  if constexpr (ACT == FRNN_ACT_GELU_TANH) return z * sigmoid_p(kGelu * z * fmaf(kGeluCube * z, z, 1.0f));
-  return z;
+__device__ __forceinline__ void act_pair(float& a, float& b) {
+  if constexpr (ACT == FRNN_ACT_RELU) {
+    a = a < 0.0f ? 0.0f : a;  // a NaN stays one
+    b = b < 0.0f ? 0.0f : b;
+  }
+  if constexpr (ACT == FRNN_ACT_SILU || ACT == FRNN_ACT_GELU_TANH) {
+    float ea = a, eb = b;  // -log2(e) w
+    if constexpr (ACT == FRNN_ACT_SILU) {
+      mul2(ea, eb, -kLog2e, -kLog2e);
+    } else {
+      mul2(ea, eb, a, b);
+      fma2(ea, eb, -kLog2e * kGelu * kGeluCube, -kLog2e * kGelu * kGeluCube, -kLog2e * kGelu, -kLog2e * kGelu);
+      mul2(ea, eb, a, b);
+    }
+    ea = exp2_fast(ea);
+    eb = exp2_fast(eb);
+    add2(ea, eb, 1.0f, 1.0f);
+    mul2(a, b, rcp_fast(ea), rcp_fast(eb));
+  }
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
@@ -133,50 +163,54 @@ __device__ __forceinline__ float act_slope(float z) {
 template <int ACT, int N>
 __device__ __forceinline__ void act_row(float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = act_value<ACT>(v[i]);
+  for (int i = 0; i < N; i += 2) act_pair<ACT>(v[i], v[i + 1]);
 }
-template <int N>
-__device__ __forceinline__ void act_row(int act, float (&v)[N]) {
-  if (act == FRNN_ACT_RELU) act_row<FRNN_ACT_RELU>(v);
-  else if (act == FRNN_ACT_SILU) act_row<FRNN_ACT_SILU>(v);
-  else if (act == FRNN_ACT_GELU_TANH) act_row<FRNN_ACT_GELU_TANH>(v);
-}
-// What the slope is taken at. Of a relu the side of zero alone counts, which a small z could lose in 16 bits.
-__device__ __forceinline__ void keep_slope(int act, const float (&v)[8], float (&z)[8]) {
+// What the slope is taken at, eight columns as fp16. Of a relu the side of zero alone counts, which a small z could lose in 16 bits.
+template <int ACT>
+__device__ __forceinline__ void keep_slope(const float* v, uint32_t (&w)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = act == FRNN_ACT_RELU ? (v[i] > 0.0f ? 1.0f : 0.0f) : v[i];
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i], b = v[2 * i + 1];
+    if constexpr (ACT == FRNN_ACT_RELU) w[i] = (a > 0.0f ? 0x3c00u : 0u) | (b > 0.0f ? 0x3c000000u : 0u);
+    else w[i] = pack_half2(a, b);
+  }
 }
 // v[i] += bias[j + i], eight columns of a row of N (a multiple of eight)
-__device__ __forceinline__ void add_bias(const ProductParams& p, int j, float (&v)[8]) {
-  if (p.bias == nullptr || j >= p.N) return;
+__device__ __forceinline__ void add_bias(const ProductParams& p, int j, float* v) {
+  if (j >= p.N) return;
   if (p.bias_bf16) {
     const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + j));
-    v[0] += bf16_lo(w.x); v[1] += bf16_hi(w.x); v[2] += bf16_lo(w.y); v[3] += bf16_hi(w.y);
-    v[4] += bf16_lo(w.z); v[5] += bf16_hi(w.z); v[6] += bf16_lo(w.w); v[7] += bf16_hi(w.w);
+    add2(v[0], v[1], bf16_lo(w.x), bf16_hi(w.x));
+    add2(v[2], v[3], bf16_lo(w.y), bf16_hi(w.y));
+    add2(v[4], v[5], bf16_lo(w.z), bf16_hi(w.z));
+    add2(v[6], v[7], bf16_lo(w.w), bf16_hi(w.w));
   } else {
     const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + j));
     const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + j + 4));
-    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    add2(v[0], v[1], a.x, a.y);
+    add2(v[2], v[3], a.z, a.w);
+    add2(v[4], v[5], b.x, b.y);
+    add2(v[6], v[7], b.z, b.w);
   }
 }
-__device__ __forceinline__ void add_bf16(const uint32_t (&w)[4], float (&v)[8]) {
+__device__ __forceinline__ void add_bf16(const uint32_t (&w)[4], float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+  for (int i = 0; i < 4; ++i) add2(v[2 * i], v[2 * i + 1], bf16_lo(w[i]), bf16_hi(w[i]));
 }
 
 // A_MN / B_MN: the operand's rows in memory run along M / N instead of K. PARTIAL: fp32 tiles of one of several parts of K, no epilogue.
-template <bool A_MN, bool B_MN, int NP, bool PARTIAL>
+template <bool A_MN, bool B_MN, int NP, bool PARTIAL, int ACT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
                const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
                const __grid_constant__ CUtensorMap z_map) {
   extern __shared__ uint8_t smem_raw[];
+  constexpr int kStages = stages_of(NP, B_MN);
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2], s_done;
   __shared__ __align__(8) uint64_t s_res[kEpiWarps][2];
   __shared__ uint32_t s_tmem_base;
   constexpr int NH = NP / 2;  // rows of B in each CTA
-  constexpr uint32_t kStageBytes = 16384u + NH * 128u, kCols = 2u * NP;
+  constexpr uint32_t kStageBytes = stage_bytes_of(NP, B_MN), kCols = NP > 128 ? 512u : 2u * NP;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(cluster_rank());  // 0: the one that issues
   const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -197,6 +231,13 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
     mbar_init(smem_u32(&s_done), 1);
     fence_mbar_init();
+  }
+  if (warp == 7 && lane == 0) {
+    tma_prefetch_desc(&a_map);
+    tma_prefetch_desc(&b_map);
+    tma_prefetch_desc(&out_map);
+    if (p.has_residual) tma_prefetch_desc(&res_map);
+    if (p.has_z) tma_prefetch_desc(&z_map);
   }
   if (warp == 9) tmem_alloc_pair(smem_u32(&s_tmem_base), kCols);
   tc_fence_before_sync();
@@ -220,15 +261,13 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
 
   if (warp == 8) {
     if (lane == 0) {
-      tma_prefetch_desc(&a_map);
-      tma_prefetch_desc(&b_map);
       uint32_t s = 0, round = 0;
       bool dead = false;
       for (long long t = pair; t < p.n_tiles && !dead; t += pairs) {
         const Tile tile = tile_at(t);
         const int ma = tile.m0 + 128 * cta, nb = tile.n0 + NH * cta;
         for (int i = tile.c_begin; i < tile.c_end; ++i) {
-          if (round > 0 && !mbar_wait_bounded<true, true>(smem_u32(&s_empty[s]), (round - 1) & 1, kLimit, abort_flag)) {
+          if (round > 0 && !mbar_wait_bounded<false, true>(smem_u32(&s_empty[s]), (round - 1) & 1, kLimit, abort_flag)) {
             atomicCAS(p.err, 0, kErrWaitEmpty);
             dead = true;
             break;
@@ -244,7 +283,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
             tma_load_2d_pair(sa, &a_map, bar, k0, ma);
           }
           if constexpr (B_MN) {
-            for (int j = 0; j < NH / 64; ++j) tma_load_2d_pair(sb + j * 8192u, &b_map, bar, nb + 64 * j, k0);
+            for (int j = 0; j < (NH + 63) / 64; ++j) tma_load_2d_pair(sb + j * 8192u, &b_map, bar, nb + 64 * j, k0);
           } else {
             tma_load_2d_pair(sb, &b_map, bar, k0, nb);
           }
@@ -256,7 +295,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         const uint32_t r = s > 0 ? round : round - 1;
         s = s > 0 ? s - 1 : kStages - 1;
         round = r;
-        dead = !mbar_wait_bounded<true, true>(smem_u32(&s_empty[s]), r & 1, kLimit, abort_flag);
+        dead = !mbar_wait_bounded<false, true>(smem_u32(&s_empty[s]), r & 1, kLimit, abort_flag);
         if (dead) atomicCAS(p.err, 0, kErrWaitEmpty);
       }
       if (dead) {  // copies in flight land before the CTA leaves
@@ -279,7 +318,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         tc_fence_after_sync();
         const uint32_t d = tbase + a * NP;
         for (int i = tile.c_begin; i < tile.c_end; ++i) {
-          if (!mbar_wait_bounded<true, true>(smem_u32(&s_full[s]), round & 1, kLimit, abort_flag)) {
+          if (!mbar_wait_bounded<false, true>(smem_u32(&s_full[s]), round & 1, kLimit, abort_flag)) {
             atomicCAS(p.err, 0, kErrWaitWx);
             dead = true;
             break;
@@ -302,60 +341,70 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       }
       // covers every MMA issued so far, also after a failed wait: tensor and shared memory stay until they are done
       umma_commit_pair_here(smem_u32(&s_done));
-      mbar_wait_bounded<true, true>(smem_u32(&s_done), 0, kLimit, nullptr);
+      mbar_wait_bounded<false, true>(smem_u32(&s_done), 0, kLimit, nullptr);
     }
   } else {
     const int q = warp & 3, half = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; columns
     constexpr int CW = PARTIAL ? 32 : 64;      // columns of a piece: 128 bytes
-    constexpr int kPieces = NH / CW;           // a warp has half of the tile's NP columns
-    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 3u * kBufBytes, zbuf = buf0 + 2u * kBufBytes;
+    constexpr int kPieces = NP / CW;           // of the tile, in turn to the two warps of a quarter
+    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 2u * kBufBytes;
     const uint32_t my_row = static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
+    // Without z the pieces take the two buffers in turn; with it z goes through the first, y through the second. The residual's
+    // piece is loaded into the buffer that y leaves from.
+    const bool z_too = !PARTIAL && ACT != FRNN_ACT_NONE && p.has_z;
     uint32_t li = 0, used = 0, res_phase = 0;  // used: pieces staged so far; res_phase: a bit per buffer
+    auto ask_residual = [&](uint32_t bi, int j, int m) {
+      const uint32_t bar = smem_u32(&s_res[warp][bi]);
+      mbar_arrive_expect_tx(bar, kBufBytes);
+      tma_load_2d(buf0 + bi * kBufBytes, &res_map, bar, j, m);
+    };
     for (long long t = pair; t < p.n_tiles; t += pairs, ++li) {
       const Tile tile = tile_at(t);
       const uint32_t a = li & 1u;
-      const int mw = tile.m0 + 128 * cta + 32 * q, j0 = tile.n0 + NH * half;
-      const bool any = mw < p.M && j0 < p.N;   // warp-uniform
+      const int mw = tile.m0 + 128 * cta + 32 * q, j0 = tile.n0;
+      const bool any = mw < p.M;   // warp-uniform
       if constexpr (!PARTIAL) {
-        if (p.has_residual && any && lane == 0) {  // both pieces, while the tensor cores work
+        if (p.has_residual && any && lane == 0) {  // while the tensor cores work
           tma_store_wait_read<0>();
+          if (z_too) {
+            if (j0 + half * CW < p.N) ask_residual(1, j0 + half * CW, mw);
+          } else {
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            if (j0 + i * CW >= p.N) break;
-            const uint32_t bi = (used + i) & 1u, bar = smem_u32(&s_res[warp][bi]);
-            mbar_arrive_expect_tx(bar, kBufBytes);
-            tma_load_2d(buf0 + bi * kBufBytes, &res_map, bar, j0 + i * CW, mw);
+            for (int i = 0; i < kPieces / 2 + kPieces % 2; ++i) {
+              const int piece = half + 2 * i;
+              if (piece < kPieces && j0 + piece * CW < p.N) ask_residual((used + i) & 1u, j0 + piece * CW, mw);
+            }
           }
         }
       }
-      const bool have = mbar_wait_warp<true>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag);
+      const bool have = mbar_wait_warp<false>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag);
       if (!have) {
         if (lane == 0) atomicCAS(p.err, 0, kErrWaitMma);
         break;
       }
       tc_fence_after_sync();
 #pragma unroll 1
-      for (int i = 0; i < kPieces; ++i) {
-        const int c = a * NP + NH * half + i * CW, j = j0 + i * CW;
-        uint32_t r[CW];
-        tmem_ld_x32(tmem_addr(tbase, 32 * q, c), *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        if constexpr (CW == 64) tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+      for (int i = half; i < kPieces; i += 2) {
+        const int c = a * NP + i * CW, j = j0 + i * CW;
+        float v[CW];
+        tmem_ld_x32(tmem_addr(tbase, 32 * q, c), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        if constexpr (CW == 64) tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
-        if (i == kPieces - 1) {  // the accumulator is in registers: the next tile but one may have it
+        if (i + 2 >= kPieces) {  // the accumulator is in registers: the next tile but one may have it
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s_acc_empty[a]), 0));
         }
         if (!any || j >= p.N) continue;
-        const uint32_t bi = used & 1u, buf = buf0 + bi * kBufBytes;
+        const uint32_t bi = z_too ? 1u : used & 1u, buf = buf0 + bi * kBufBytes + my_row;
         ++used;
         if constexpr (PARTIAL) {
           if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const uint32_t w[4] = {r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]};
-            st_shared_v4(buf + my_row + ((k ^ sw) << 4), w);
+            const uint32_t w[4] = {__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])};
+            st_shared_v4(buf + ((k ^ sw) << 4), w);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -364,49 +413,54 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
             tma_store_commit();
           }
         } else {
+          if (p.bias != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
+          }
+          if (lane == 0) {
+            if (z_too) tma_store_wait_read<0>();
+            else if (!p.has_residual) tma_store_wait_read<1>();
+          }
+          __syncwarp();
+          if (z_too) {
+            if (p.has_residual && i >= 2 && lane == 0) ask_residual(1, j, mw);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t w[4];
+              keep_slope<ACT>(&v[8 * k], w);
+              st_shared_v4(buf0 + my_row + ((k ^ sw) << 4), w);
+            }
+          }
+          act_row<ACT>(v);
           if (p.has_residual) {
             if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][bi]), (res_phase >> bi) & 1u, kLimit, abort_flag)) {
               if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
             }
             res_phase ^= 1u << bi;
-            if (p.has_z && lane == 0) tma_store_wait_read<0>();
-          } else if (lane == 0) {
-            if (p.has_z) tma_store_wait_read<0>();
-            else tma_store_wait_read<1>();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t w[4];
+              ld_shared_v4(buf + ((k ^ sw) << 4), w);
+              add_bf16(w, &v[8 * k]);
+            }
           }
-          __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const uint32_t at = my_row + ((k ^ sw) << 4);
-            float v[8], zv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[8 * k + e]);
-            add_bias(p, j + 8 * k, v);
-            if (p.has_z) {
-              keep_slope(p.act, v, zv);
-              const uint32_t w[4] = {pack_half2(zv[0], zv[1]), pack_half2(zv[2], zv[3]), pack_half2(zv[4], zv[5]), pack_half2(zv[6], zv[7])};
-              st_shared_v4(zbuf + at, w);
-            }
-            act_row(p.act, v);
-            if (p.has_residual) {
-              uint32_t w[4];
-              ld_shared_v4(buf + at, w);
-              add_bf16(w, v);
-            }
-            const uint32_t w[4] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-            st_shared_v4(buf + at, w);
+            const float* f = &v[8 * k];
+            const uint32_t w[4] = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+            st_shared_v4(buf + ((k ^ sw) << 4), w);
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             tma_store_2d(&out_map, buf, j, mw);
-            if (p.has_z) tma_store_2d(&z_map, zbuf, j, mw);
+            if (z_too) tma_store_2d(&z_map, buf0, j, mw);
             tma_store_commit();
           }
         }
       }
     }
-    if (lane == 0) tma_store_wait<0>();
+    if (lane == 0) tma_store_wait_read<0>();  // the staging buffers are read; the end of the kernel completes the writes
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -415,28 +469,28 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
 }
 
 // out = epilogue(sum over parts of work), eight columns of a row to a thread.
+template <int ACT>
 __global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p, const float* __restrict__ work, int parts,
                                                            const __nv_bfloat16* __restrict__ residual, __nv_bfloat16* __restrict__ out,
-                                                           __half* __restrict__ z) {
+                                                           uint4* __restrict__ z) {
   const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 8, n = static_cast<long long>(p.M) * p.N;
   if (i >= n) return;
   float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  for (int s = 0; s < parts; ++s) {
+  ld_f32_vec<8>(work + i, v);
+#pragma unroll 4
+  for (int s = 1; s < parts; ++s) {
     float w[8];
     ld_f32_vec<8>(work + s * n + i, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += w[e];
   }
-  add_bias(p, static_cast<int>(i % p.N), v);
+  if (p.bias != nullptr) add_bias(p, static_cast<int>(i % p.N), v);
   if (z != nullptr) {
-    float zv[8];
-    keep_slope(p.act, v, zv);
-    *reinterpret_cast<uint4*>(z + i) =
-        make_uint4(pack_half2(zv[0], zv[1]), pack_half2(zv[2], zv[3]), pack_half2(zv[4], zv[5]), pack_half2(zv[6], zv[7]));
+    uint32_t w[4];
+    keep_slope<ACT>(v, w);
+    z[i / 8] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  act_row(p.act, v);
+  act_row<ACT>(v);
   if (residual != nullptr) {
     const uint4 r = __ldg(reinterpret_cast<const uint4*>(residual + i));
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -516,14 +570,14 @@ Cut choose_cut(long long M, long long N, long long K) {
   const long long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, mt = (M + 255) / 256, chunks = (K + kKC - 1) / kKC;
   Cut best{};
   double best_t = 0;
-  for (int np = 256; np >= 128; np /= 2) {
+  for (int np = 256; np >= 128; np -= 64) {
     const long long tiles = mt * ((N + np - 1) / np);
     for (long long parts = 1; parts <= 16 && parts <= chunks; ++parts) {
       const long long cpp = (chunks + parts - 1) / parts;
       if ((chunks + cpp - 1) / cpp != parts) continue;
       const long long waves = (tiles * parts + pairs - 1) / pairs;
       // cycles: 64 k's of a tile, filling and draining, the pass over partial sums (4 bytes written and read)
-      double t = static_cast<double>(waves) * cpp * (np == 256 ? 520 : 300) + 3000;
+      double t = static_cast<double>(waves) * cpp * (np == 256 ? 600 : np == 192 ? 480 : 400) + 3000;
       if (parts > 1) t += 5000 + static_cast<double>(M) * N * parts * 8 / 2500;
       if (best.np == 0 || t < best_t) {
         best = {np, static_cast<int>(parts), static_cast<int>(cpp)};
@@ -544,15 +598,25 @@ int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long lo
   return make_tensor_map(map, base, elem, 2, dims, box, true);
 }
 
-template <bool A_MN, bool B_MN, int NP, bool PARTIAL>
+template <bool A_MN, bool B_MN, int NP, bool PARTIAL, int ACT>
 int launch_kernel(const ProductParams& p, const CUtensorMap (&maps)[5], cudaStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, PARTIAL>);
-  cudaError_t e = raise_limits(kern, kSmem, false);
+  const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, PARTIAL, ACT>);
+  cudaError_t e = raise_limits(kern, smem_of(NP, B_MN), false);
   if (e != cudaSuccess) return static_cast<int>(e);
   const long long pairs = sm_count() / 2;
   const unsigned grid = 2u * static_cast<unsigned>(p.n_tiles < pairs ? p.n_tiles : pairs);
-  product_kernel<A_MN, B_MN, NP, PARTIAL><<<grid, kThreads, kSmem, s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
+  product_kernel<A_MN, B_MN, NP, PARTIAL, ACT><<<grid, kThreads, smem_of(NP, B_MN), s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
   return static_cast<int>(cudaGetLastError());
+}
+// The gradients' products have no epilogue.
+template <bool A_MN, bool B_MN, int NP>
+int launch_act(const ProductParams& p, const CUtensorMap (&maps)[5], cudaStream_t s) {
+  if constexpr (!A_MN && !B_MN) {
+    if (p.act == FRNN_ACT_RELU) return launch_kernel<false, false, NP, false, FRNN_ACT_RELU>(p, maps, s);
+    if (p.act == FRNN_ACT_SILU) return launch_kernel<false, false, NP, false, FRNN_ACT_SILU>(p, maps, s);
+    if (p.act == FRNN_ACT_GELU_TANH) return launch_kernel<false, false, NP, false, FRNN_ACT_GELU_TANH>(p, maps, s);
+  }
+  return launch_kernel<A_MN, B_MN, NP, false, FRNN_ACT_NONE>(p, maps, s);
 }
 
 // C [M][N] = A . B with the epilogue of `p` (bias, act); A [M][K] or, A_MN, [K][M]; B [N][K] or, B_MN, [K][N].
@@ -577,11 +641,18 @@ int product_launch(ProductParams p, const void* A, const void* B, long long M, l
     rc = make_tensor_map(&maps[2], work, 4, 3, dims, box, true);
     if (rc != 0) return rc;
     maps[3] = maps[4] = maps[2];
-    rc = cut.np == 256 ? launch_kernel<A_MN, B_MN, 256, true>(p, maps, s) : launch_kernel<A_MN, B_MN, 128, true>(p, maps, s);
+    rc = cut.np == 256   ? launch_kernel<A_MN, B_MN, 256, true, FRNN_ACT_NONE>(p, maps, s)
+         : cut.np == 192 ? launch_kernel<A_MN, B_MN, 192, true, FRNN_ACT_NONE>(p, maps, s)
+                         : launch_kernel<A_MN, B_MN, 128, true, FRNN_ACT_NONE>(p, maps, s);
     if (rc != 0) return rc;
-    const long long threads = M * N / 8;
-    product_join_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p, work, cut.parts, static_cast<const __nv_bfloat16*>(residual),
-                                                                                   static_cast<__nv_bfloat16*>(out), static_cast<__half*>(z));
+    const unsigned blocks = static_cast<unsigned>((M * N / 8 + 255) / 256);
+    const auto* r = static_cast<const __nv_bfloat16*>(residual);
+    auto* o = static_cast<__nv_bfloat16*>(out);
+    auto* keep = static_cast<uint4*>(z);
+    if (p.act == FRNN_ACT_RELU) product_join_kernel<FRNN_ACT_RELU><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
+    else if (p.act == FRNN_ACT_SILU) product_join_kernel<FRNN_ACT_SILU><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
+    else if (p.act == FRNN_ACT_GELU_TANH) product_join_kernel<FRNN_ACT_GELU_TANH><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
+    else product_join_kernel<FRNN_ACT_NONE><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
     return static_cast<int>(cudaGetLastError());
   }
   rc = map_2d(&maps[2], out, 2, N, M, 64, 32);
@@ -590,7 +661,9 @@ int product_launch(ProductParams p, const void* A, const void* B, long long M, l
   if (rc != 0) return rc;
   if (residual == nullptr) maps[3] = maps[2];
   if (z == nullptr) maps[4] = maps[2];
-  return cut.np == 256 ? launch_kernel<A_MN, B_MN, 256, false>(p, maps, s) : launch_kernel<A_MN, B_MN, 128, false>(p, maps, s);
+  return cut.np == 256   ? launch_act<A_MN, B_MN, 256>(p, maps, s)
+         : cut.np == 192 ? launch_act<A_MN, B_MN, 192>(p, maps, s)
+                         : launch_act<A_MN, B_MN, 128>(p, maps, s);
 }
 
 bool bad_sizes(int64_t rows, int outputs, int inputs) { return rows < 1 || outputs < 1 || inputs < 1; }

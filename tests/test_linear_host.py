@@ -48,7 +48,7 @@ def test_plan():
     assert (p.gates, p.tiles, p.tile_steps * p.tiles) == (2, 8, 1024)
     assert p.starts_bytes == 4 * 8 * 7 * 768 and p.dbpart_bytes == 4 * 8 * 8 * 2 * 768
     assert p.exchange_bytes >= 8 * 8 * 768 * 8
-    one = _lib.linear_plan("lstm", 1, p.tile_steps, 1, 7)
+    one = _lib.linear_plan("lstm", 1, _lib.linear_plan("lstm", 1, 1, 1, 1).tile_steps, 1, 7)
     assert (one.gates, one.tiles, one.exchange_bytes, one.starts_bytes, one.dbpart_bytes) == (4, 1, 0, 0, 0)
     lib = _lib.load()
     for a, rc in (((2, 1, 1, 1, 1), -1), ((0, 0, 1, 1, 1), -5), ((0, 1, 1, 1, 0), -5), ((0, 1, 1, 2 ** 16, 2 ** 16), -2), ((1, 2 ** 30, 2 ** 10, 1, 1), -2)):
