@@ -48,10 +48,99 @@ struct LinParams {
   float* d_initial;       // [B][ND] or null
 };
 
-// VEC neighbouring values of a row, as they lie in memory.
-template <int VEC, bool BF16>
+// N fp32 values of neighbouring channels; two share an instruction where N is even.
+template <int N>
+struct Vec {
+  float v[N];
+  __device__ __forceinline__ float& operator[](int i) { return v[i]; }
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+};
+template <int N>
+__device__ __forceinline__ Vec<N> splat(float x) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = x;
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> fma_(const Vec<N>& a, const Vec<N>& b, const Vec<N>& c) {
+  Vec<N> r;
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n"
+          " mov.b64 {%0, %1}, x;\n}"
+          : "=f"(r.v[i]), "=f"(r.v[i + 1])
+          : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]), "f"(c.v[i]), "f"(c.v[i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = __fmaf_rn(a.v[i], b.v[i], c.v[i]);
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> mul_(const Vec<N>& a, const Vec<N>& b) {
+  Vec<N> r;
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+          : "=f"(r.v[i]), "=f"(r.v[i + 1])
+          : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = __fmul_rn(a.v[i], b.v[i]);
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> add_(const Vec<N>& a, const Vec<N>& b) {
+  Vec<N> r;
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+          : "=f"(r.v[i]), "=f"(r.v[i + 1])
+          : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = __fadd_rn(a.v[i], b.v[i]);
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> exp2_(const Vec<N>& a) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = exp2_fast(a.v[i]);
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> rcp_(const Vec<N>& a) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = rcp_fast(a.v[i]);
+  return r;
+}
+// min that keeps a NaN
+template <int N>
+__device__ __forceinline__ Vec<N> min_(const Vec<N>& a, float b) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm("min.NaN.f32 %0, %1, %2;" : "=f"(r.v[i]) : "f"(a.v[i]), "f"(b));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> load_(const float* p) {
+  Vec<N> r;
+  ld_f32_vec<N>(p, r.v);
+  return r;
+}
+
+// N neighbouring values of a row, as they lie in memory.
+template <int N, bool BF16>
 struct Pack {
-  static constexpr int kBytes = VEC * (BF16 ? 2 : 4);
+  static constexpr int kBytes = N * (BF16 ? 2 : 4);
   uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -70,20 +159,25 @@ struct Pack {
       w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     }
   }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (BF16) return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
-    else return __uint_as_float(w[i]);
+  __device__ __forceinline__ Vec<N> get() const {
+    Vec<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (BF16) r.v[i] = __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+      else r.v[i] = __uint_as_float(w[i]);
+    }
+    return r;
   }
-  // one rounding, to the type of Wx, of a value computed in fp32
-  __device__ __forceinline__ void set(const float* v) {
+  // one rounding, to the type of Wx, of values computed in fp32
+  __device__ __forceinline__ void set(const Vec<N>& v) {
     if constexpr (!BF16) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(v[i]);
-    } else if constexpr (VEC == 1) {
-      w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+      for (int i = 0; i < N; ++i) w[i] = __float_as_uint(v.v[i]);
+    } else if constexpr (N == 1) {
+      w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v.v[0]));
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; i += 2) w[i / 2] = pack_bf16x2(v[i], v[i + 1]);
+      for (int i = 0; i < N; i += 2) w[i / 2] = pack_bf16x2(v.v[i], v.v[i + 1]);
     }
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
@@ -94,49 +188,46 @@ struct Pack {
   }
 };
 
-// min that keeps a NaN
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 constexpr float kLog2e = 1.4426950408889634f;
 // sigmoid(x) and tanh(y) from a = -log2(e) x and b = -2 log2(e) y with one reciprocal for both: 1 / (1 + 2^a) and
 // (1 - 2^b) / (1 + 2^b). The bounds keep the product of the denominators in range; past them the results are 0 and -1 anyway.
-__device__ __forceinline__ void sigmoid_tanh(float a, float b, float& s, float& t) {
-  const float ea = exp2_fast(min_nan(a, 80.0f)), eb = exp2_fast(min_nan(b, 43.0f)), da = 1.0f + ea, db = 1.0f + eb, r = rcp_fast(da * db);
-  s = db * r;
-  t = (1.0f - eb) * (da * r);
+template <int N>
+__device__ __forceinline__ void sigmoid_tanh(const Vec<N>& a, const Vec<N>& b, Vec<N>& s, Vec<N>& t) {
+  const Vec<N> one = splat<N>(1.0f), eb = exp2_(min_(b, 43.0f)), da = add_(one, exp2_(min_(a, 80.0f))), db = add_(one, eb), r = rcp_(mul_(da, db));
+  s = mul_(db, r);
+  t = mul_(fma_(eb, splat<N>(-1.0f), one), mul_(da, r));
 }
-__device__ __forceinline__ float sigmoid_times_tanh(float a, float b) {
-  const float ea = exp2_fast(min_nan(a, 80.0f)), eb = exp2_fast(min_nan(b, 43.0f));
-  return (1.0f - eb) * rcp_fast((1.0f + ea) * (1.0f + eb));
+template <int N>
+__device__ __forceinline__ Vec<N> sigmoid_times_tanh(const Vec<N>& a, const Vec<N>& b) {
+  const Vec<N> one = splat<N>(1.0f), eb = exp2_(min_(b, 43.0f)), da = add_(one, exp2_(min_(a, 80.0f)));
+  return mul_(fma_(eb, splat<N>(-1.0f), one), rcp_(mul_(da, add_(one, eb))));
 }
 
-// Gates arrive as scale(g) (Wx + b): the factor that the exponentials want goes into one fused multiply-add with the bias.
+// Gates arrive as scale(g) (Wx + b): the factor that the exponentials want goes into one fused multiply-add with the bias. What a
+// step does is kept as n = -u and v: c + v - u c = fma(n, c, c + v).
 // kTile: steps of a tile. The LSTM's backward pass holds five values per step and channel: 64 steps leave room for two CTAs.
 template <int CELL> struct LinCell;
 template <> struct LinCell<FRNN_LINEAR_LEAKY> {
   static constexpr int G = 2, kTile = 128;
-  static __device__ __forceinline__ constexpr float scale(int g) { return g == 0 ? kLog2e : 1.0f; }
-  static __device__ __forceinline__ void gates(const float* x, float& u, float& v) {
-    u = rcp_fast(1.0f + exp2_fast(x[0]));
-    v = u * x[1];
+  static __device__ __forceinline__ constexpr float scale(int g) { return g == 0 ? kLog2e : -1.0f; }  // the second gate is -z
+  template <int N>
+  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& n, Vec<N>& v) {
+    n = rcp_(fma_(exp2_(x[0]), splat<N>(-1.0f), splat<N>(-1.0f)));
+    v = mul_(n, x[1]);
   }
-  static __device__ __forceinline__ float hidden(float, float c) { return c; }
 };
 template <> struct LinCell<FRNN_LINEAR_LSTM> {
   static constexpr int G = 4, kTile = 64;
   static __device__ __forceinline__ constexpr float scale(int g) { return g == 1 ? kLog2e : (g == 2 ? -2.0f * kLog2e : -kLog2e); }
-  static __device__ __forceinline__ void gates(const float* x, float& u, float& v) {
-    u = rcp_fast(1.0f + exp2_fast(x[1]));
+  template <int N>
+  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& n, Vec<N>& v) {
+    n = rcp_(fma_(exp2_(x[1]), splat<N>(-1.0f), splat<N>(-1.0f)));
     v = sigmoid_times_tanh(x[0], x[2]);
   }
-  static __device__ __forceinline__ float hidden(float o, float c) { return sigmoid_times_tanh(o, -2.0f * kLog2e * c); }
 };
 
-// c -> f c + v
-__device__ __forceinline__ float lin_step(float u, float v, float c) { return fmaf(-u, c, c + v); }
+template <int N>
+__device__ __forceinline__ Vec<N> lin_step(const Vec<N>& n, const Vec<N>& v, const Vec<N>& c) { return fma_(n, c, add_(c, v)); }
 
 template <int VEC>
 struct Lanes {
@@ -257,10 +348,22 @@ __device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x
   return carry;
 }
 
-// The tile of this CTA: from the counter where tiles wait on one another.
-__device__ __forceinline__ int lin_tile(const LinParams& p, int* shared) {
-  if (p.n_tiles == 1) return static_cast<int>(blockIdx.x);
-  if (threadIdx.x == 0) *shared = atomicAdd(reinterpret_cast<int*>(p.exchange), 1) + 1;  // it starts at -1
+// The tile of this CTA, from the counter where tiles wait on one another: k, row, b, channel block, and the row's length. One
+// thread divides for all.
+struct TileId { int k, row, b, cg, len; };
+__device__ __forceinline__ TileId lin_tile(const LinParams& p, TileId* shared) {
+  if (threadIdx.x == 0) {
+    int id = static_cast<int>(blockIdx.x);
+    if (p.n_tiles > 1) id = atomicAdd(reinterpret_cast<int*>(p.exchange), 1) + 1;  // it starts at -1
+    TileId t;
+    const int rows = p.B * p.n_cg;
+    t.k = id / rows;
+    t.row = id - t.k * rows;
+    t.b = t.row / p.n_cg;
+    t.cg = t.row - t.b * p.n_cg;
+    t.len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + t.b), 0), p.T);
+    *shared = t;
+  }
   __syncthreads();
   return *shared;
 }
@@ -271,11 +374,6 @@ struct Shared {
   float a[NW][CW], h[NW][CW], start[NW][CW];
   float2 prev[kGroup - 1][CW];
 };
-
-template <int VEC>
-__device__ __forceinline__ void ld_vec(const float* p, float (&v)[VEC]) { ld_f32_vec<VEC>(p, v); }
-template <int VEC>
-__device__ __forceinline__ void st_vec(float* p, const float (&v)[VEC]) { st_f32_vec<VEC>(p, v); }
 
 // From the maps of the CTA's warps to the value that each of them starts from; warps count backwards in reverse time. `first` [B][ND]
 // (null: zeros) is what the row starts from; done(state, channel, carry, end) is called per channel with its place in [B][ND], what
@@ -327,21 +425,20 @@ template <int VEC, int L, int TILE>
 struct Place {
   int k, row, b, c0, chl, ch, warp, span, t0, len;
   bool ok, whole;  // ok: the channels exist; whole: and so do all steps of the warp
-  __device__ __forceinline__ Place(const LinParams& p, int id, bool reverse) {
+  __device__ __forceinline__ Place(const LinParams& p, const TileId& id, bool reverse) {
     using W = Lanes<VEC>;
-    const int lane = threadIdx.x & 31, rows = p.B * p.n_cg;
+    const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
-    k = id / rows;
-    row = id - k * rows;
-    if (reverse) k = p.n_tiles - 1 - k;
-    b = row / p.n_cg;
-    c0 = (row - b * p.n_cg) * W::kChannels;
+    k = reverse ? p.n_tiles - 1 - id.k : id.k;
+    row = id.row;
+    b = id.b;
+    c0 = id.cg * W::kChannels;
     span = lane / W::kRow;
     chl = (lane % W::kRow) * VEC;
     ch = c0 + chl;
     t0 = k * TILE + (warp * W::kSpans + span) * L;
     ok = ch < p.ND;
-    len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
+    len = id.len;
     whole = k * TILE + (warp + 1) * W::kSpans * L <= len && c0 + W::kChannels <= p.ND;
   }
   __device__ __forceinline__ bool valid(int l) const { return ok && t0 + l < len; }
@@ -350,65 +447,61 @@ struct Place {
 // The maps of the warp's spans, one to a lane, become those of what lies in front of each (behind, in reverse time); that of the whole
 // warp goes to (a, h) in shared memory.
 template <int VEC, bool REVERSE>
-__device__ __forceinline__ void join_spans(int span, float (&A)[VEC], float (&H)[VEC], float* a, float* h) {
+__device__ __forceinline__ void join_spans(int span, Vec<VEC>& A, Vec<VEC>& H, float* a, float* h) {
   using W = Lanes<VEC>;
-  auto from = [&](float v, int o) {
-    return REVERSE ? __shfl_down_sync(0xffffffffu, v, o * W::kRow) : __shfl_up_sync(0xffffffffu, v, o * W::kRow);
+  auto from = [&](const Vec<VEC>& v, int o) {
+    Vec<VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      r[i] = REVERSE ? __shfl_down_sync(0xffffffffu, v[i], o * W::kRow) : __shfl_up_sync(0xffffffffu, v[i], o * W::kRow);
+    return r;
   };
   const int at = REVERSE ? W::kSpans - 1 - span : span;  // place in the order of the scan
 #pragma unroll
   for (int o = 1; o < W::kSpans; o *= 2) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float pa = from(A[i], o), ph = from(H[i], o);
-      if (at >= o) {
-        H[i] = fmaf(A[i], ph, H[i]);
-        A[i] *= pa;
-      }
+    const Vec<VEC> pa = from(A, o), ph = from(H, o);
+    if (at >= o) {
+      H = fma_(A, ph, H);
+      A = mul_(A, pa);
     }
   }
   if (at == W::kSpans - 1) {
-    st_vec<VEC>(a, A);
-    st_vec<VEC>(h, H);
+    st_f32_vec<VEC>(a, A.v);
+    st_f32_vec<VEC>(h, H.v);
   }
   if constexpr (W::kSpans > 1) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      A[i] = from(A[i], 1);
-      H[i] = from(H[i], 1);
-    }
+    A = from(A, 1);
+    H = from(H, 1);
   }
   if (at == 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) { A[i] = 1.0f; H[i] = 0.0f; }
+    A = splat<VEC>(1.0f);
+    H = splat<VEC>(0.0f);
   }
 }
 
 template <int CELL, int VEC>
-__device__ __forceinline__ void load_bias(const LinParams& p, bool ok, int ch, float (&bias)[LinCell<CELL>::G][VEC]) {
+__device__ __forceinline__ void load_bias(const LinParams& p, bool ok, int ch, Vec<VEC> (&bias)[LinCell<CELL>::G]) {
 #pragma unroll
   for (int g = 0; g < LinCell<CELL>::G; ++g) {
-    if (ok) {
-      ld_vec<VEC>(p.bias + static_cast<long long>(g) * p.ND + ch, bias[g]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) bias[g][i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) bias[g][i] *= LinCell<CELL>::scale(g);
+    bias[g] = ok ? load_<VEC>(p.bias + static_cast<long long>(g) * p.ND + ch) : splat<VEC>(0.0f);
+    bias[g] = mul_(bias[g], splat<VEC>(LinCell<CELL>::scale(g)));
   }
+}
+template <int CELL, int VEC, bool BF16>
+__device__ __forceinline__ Vec<VEC> scaled(const Pack<VEC, BF16>& raw, const Vec<VEC>& bias, int g) {
+  return fma_(raw.get(), splat<VEC>(LinCell<CELL>::scale(g)), bias);
 }
 
 template <int CELL, int VEC, int L, int NW, int MIN_CTAS, bool BF16>
 __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const LinParams p) {
   using W = Lanes<VEC>;
   using Cell = LinCell<CELL>;
+  using V = Vec<VEC>;
   constexpr int G = Cell::G, CW = W::kChannels;
   static_assert(NW * W::kSpans * L == Cell::kTile, "a full CTA covers a tile");
   __shared__ __align__(16) Shared<CW, NW> s;
-  __shared__ int s_tile;
-  const int id = lin_tile(p, &s_tile);
-  const Place<VEC, L, Cell::kTile> at(p, id, false);
+  __shared__ TileId s_tile;
+  const Place<VEC, L, Cell::kTile> at(p, lin_tile(p, &s_tile), false);
 
   const size_t es = BF16 ? 2 : 4, gate = static_cast<size_t>(p.ND) * es;
   const uint8_t* from = static_cast<const uint8_t*>(p.wx) + ((static_cast<size_t>(at.b) * p.T + at.t0) * G * p.ND + at.ch) * es;
@@ -417,7 +510,10 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
-      for (int g = 0; g < G; ++g) raw[l][g].load(from + (l * G + g) * gate);
+      for (int g = 0; g < G; ++g) {
+        raw[l][g].load(from);
+        from += gate;
+      }
   } else {
 #pragma unroll
     for (int l = 0; l < L; ++l)
@@ -429,43 +525,33 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   }
   Fetched<CW, NW> got;
   if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), at.k, min(CW, p.ND - at.c0));
-  float bias[G][VEC];
+  V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  // the maps of this thread's steps up to each of them
-  float A[L][VEC], H[L][VEC], a[VEC], h[VEC];
+  // The maps of this thread's steps up to each of them. The leaky cell keeps only the last one, and its gates as they came in: making
+  // them again costs less than the room for twice as many warps.
+  constexpr int KEEP = CELL == FRNN_LINEAR_LSTM ? L : 1;
+  V A[KEEP], H[KEEP], a, h;
+  auto gates = [&](int l, V& n, V& v) {
+    V x[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
+    Cell::gates(x, n, v);
+    if (!at.whole && !at.valid(l)) n = v = splat<VEC>(0.0f);  // a step behind the end of a sequence leaves its state alone
+  };
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float x[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = fmaf(raw[l][g].get(i), Cell::scale(g), bias[g][i]);
-      Cell::gates(x, A[l][i], H[l][i]);  // u and v
+    V n, v;
+    gates(l, n, v);
+    if (l == 0) {
+      a = add_(splat<VEC>(1.0f), n);
+      h = v;
+    } else {
+      h = lin_step(n, v, h);
+      a = fma_(n, a, a);
     }
+    if constexpr (KEEP > 1) { A[l] = a; H[l] = h; }
   }
-  if (!at.whole) {  // a step behind the end of a sequence leaves its state alone
-#pragma unroll
-    for (int l = 0; l < L; ++l)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (!at.valid(l)) A[l][i] = H[l][i] = 0.0f;
-  }
-#pragma unroll
-  for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float u = A[l][i], v = H[l][i];
-      if (l == 0) {
-        A[0][i] = 1.0f - u;
-      } else {
-        H[l][i] = lin_step(u, v, H[l - 1][i]);
-        A[l][i] = fmaf(-u, A[l - 1][i], A[l - 1][i]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) { a[i] = A[L - 1][i]; h[i] = H[L - 1][i]; }
   join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
   lin_join<CW, NW, false>(p, at.row, at.k, p.initial, s, got, [&](long long state, int channel, float carry, float end) {
@@ -473,28 +559,27 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
     if (at.k == p.n_tiles - 1) p.last[state] = end;
   });
   if (!at.ok) return;
-  float c[VEC];
-  ld_vec<VEC>(&s.start[at.warp][at.chl], c);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = fmaf(a[i], c[i], h[i]);
-  const size_t step = static_cast<size_t>(p.ND) * es;
+  V c = fma_(a, load_<VEC>(&s.start[at.warp][at.chl]), h);
   uint8_t* to = static_cast<uint8_t*>(p.hidden) + ((static_cast<size_t>(at.b) * p.T + at.t0) * p.ND + at.ch) * es;
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    float out[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float o = G == 4 ? fmaf(raw[l][G - 1].get(i), Cell::scale(G - 1), bias[G - 1][i]) : 0.0f;
-      out[i] = Cell::hidden(o, fmaf(A[l][i], c[i], H[l][i]));
+    V out;
+    if constexpr (KEEP > 1) {
+      out = fma_(A[l], c, H[l]);
+      out = sigmoid_times_tanh(scaled<CELL>(raw[l][G - 1], bias[G - 1], G - 1), mul_(out, splat<VEC>(-2.0f * kLog2e)));
+    } else {
+      V n, v;
+      gates(l, n, v);
+      out = c = lin_step(n, v, c);
     }
     if (!at.whole) {
       if (at.t0 + l >= p.T) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = at.valid(l) ? out[i] : 0.0f;
+      if (!at.valid(l)) out = splat<VEC>(0.0f);
     }
     Pack<VEC, BF16> w;
     w.set(out);
-    w.store(to + l * step);
+    w.store(to);
+    to += gate;
   }
 }
 
@@ -502,17 +587,18 @@ template <int CELL, int VEC, int L, int NW, int MIN_CTAS, bool BF16>
 __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const LinParams p) {
   using W = Lanes<VEC>;
   using Cell = LinCell<CELL>;
+  using V = Vec<VEC>;
+  constexpr bool LSTM = CELL == FRNN_LINEAR_LSTM;
   constexpr int G = Cell::G, CW = W::kChannels;
   static_assert(NW * W::kSpans * L == Cell::kTile, "a full CTA covers a tile");
   __shared__ __align__(16) Shared<CW, NW> s;
-  __shared__ __align__(16) float s_db[NW][G][CW];  // first the maps of the recomputed states and what their warps start from
-  __shared__ int s_tile;
+  __shared__ __align__(16) float s_db[NW][G][CW];  // first the maps of the recomputed states
+  __shared__ TileId s_tile;
   static_assert(G >= 2, "room for the maps");
   float(*f_a)[CW] = reinterpret_cast<float(*)[CW]>(&s_db[0][0][0]);  // [NW][CW]
   float(*f_h)[CW] = f_a + NW;
   const int tid = threadIdx.x, nw = blockDim.x >> 5;
-  const int id = lin_tile(p, &s_tile);
-  const Place<VEC, L, Cell::kTile> at(p, id, true);
+  const Place<VEC, L, Cell::kTile> at(p, lin_tile(p, &s_tile), true);
   const int kr = p.n_tiles - 1 - at.k;  // in the order of the scan
 
   const size_t es = BF16 ? 2 : 4, row_bytes = static_cast<size_t>(p.ND) * es, first = static_cast<size_t>(at.b) * p.T + at.t0;
@@ -524,8 +610,12 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
 #pragma unroll
     for (int l = 0; l < L; ++l) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) raw[l][g].load(from + (l * G + g) * row_bytes);
-      raw_dh[l].load(from_dh + l * row_bytes);
+      for (int g = 0; g < G; ++g) {
+        raw[l][g].load(from);
+        from += row_bytes;
+      }
+      raw_dh[l].load(from_dh);
+      from_dh += row_bytes;
     }
   } else {
 #pragma unroll
@@ -553,43 +643,34 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     if (at.k > 0) before[r] = __ldg(p.starts + (static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + at.c0 + c);
     else if (p.initial != nullptr) before[r] = __ldg(p.initial + static_cast<long long>(at.b) * p.ND + at.c0 + c);
   }
-  float bias[G][VEC];
+  V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  // u; the state in front of each step; the LSTM's i and z
-  float u[L][VEC], prev[L][VEC], si[G == 4 ? L : 1][VEC], tz[G == 4 ? L : 1][VEC], A[VEC], H[VEC];
+  // n = -u; the state in front of each step; the LSTM's i and z
+  V n[L], prev[L], si[LSTM ? L : 1], tz[LSTM ? L : 1];
 #pragma unroll
   for (int l = 0; l < L; ++l) {
+    V x[G];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float x[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) x[g] = fmaf(raw[l][g].get(i), Cell::scale(g), bias[g][i]);
-      if constexpr (G == 4) {
-        u[l][i] = rcp_fast(1.0f + exp2_fast(x[1]));
-        sigmoid_tanh(x[0], x[2], si[l][i], tz[l][i]);
-        prev[l][i] = si[l][i] * tz[l][i];
-      } else {
-        Cell::gates(x, u[l][i], prev[l][i]);  // v, until the states are known
-      }
+    for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
+    if constexpr (LSTM) {
+      n[l] = rcp_(fma_(exp2_(x[1]), splat<VEC>(-1.0f), splat<VEC>(-1.0f)));
+      sigmoid_tanh(x[0], x[2], si[l], tz[l]);
+      prev[l] = mul_(si[l], tz[l]);
+    } else {
+      Cell::gates(x, n[l], prev[l]);  // v, until the states are known
     }
   }
   if (!at.whole) {
 #pragma unroll
     for (int l = 0; l < L; ++l)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (!at.valid(l)) u[l][i] = prev[l][i] = 0.0f;
+      if (!at.valid(l)) n[l] = prev[l] = splat<VEC>(0.0f);
   }
+  V A = add_(splat<VEC>(1.0f), n[0]), H = prev[0];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    A[i] = 1.0f - u[0][i];
-    H[i] = prev[0][i];
-#pragma unroll
-    for (int l = 1; l < L; ++l) {
-      H[i] = lin_step(u[l][i], prev[l][i], H[i]);
-      A[i] = fmaf(-u[l][i], A[i], A[i]);
-    }
+  for (int l = 1; l < L; ++l) {
+    H = lin_step(n[l], prev[l], H);
+    A = fma_(n[l], A, A);
   }
   join_spans<VEC, false>(at.span, A, H, &f_a[at.warp][at.chl], &f_h[at.warp][at.chl]);
   __syncthreads();
@@ -605,44 +686,29 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     }
   }
   __syncthreads();
-  float c[VEC], db[G][VEC];
+  V c = at.ok ? load_<VEC>(&s.start[at.warp][at.chl]) : splat<VEC>(0.0f), db[G];
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) db[g][i] = 0.0f;
-  if (at.ok) {
-    ld_vec<VEC>(&s.start[at.warp][at.chl], c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) c[i] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = fmaf(A[i], c[i], H[i]);
+  for (int g = 0; g < G; ++g) db[g] = splat<VEC>(0.0f);
+  c = fma_(A, c, H);
   // the gradient of each state through its hidden state; the output gate's is done with
-  float dc[G == 4 ? L : 1][VEC];
-  auto d_state = [&](int l, int i) {
-    if constexpr (G == 4) return dc[l][i];
-    else return raw_dh[l].get(i);
+  V dc[LSTM ? L : 1] = {};
+  auto d_state = [&](int l) {
+    if constexpr (LSTM) return dc[l];
+    else return raw_dh[l].get();
   };
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    float d_o[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float v = prev[l][i];
-      prev[l][i] = c[i];
-      c[i] = lin_step(u[l][i], v, c[i]);
-      if constexpr (G == 4) {
-        float o, tc;
-        sigmoid_tanh(fmaf(raw[l][3].get(i), Cell::scale(3), bias[3][i]), -2.0f * kLog2e * c[i], o, tc);
-        const float dh_o = raw_dh[l].get(i) * o;
-        dc[l][i] = dh_o * fmaf(-tc, tc, 1.0f);
-        d_o[i] = dh_o * tc * (1.0f - o);
-        if (!at.whole && !at.valid(l)) dc[l][i] = d_o[i] = 0.0f;
-        db[3][i] += d_o[i];
-      }
-    }
-    if constexpr (G == 4) {
+    const V v = prev[l];
+    prev[l] = c;
+    c = lin_step(n[l], v, c);
+    if constexpr (LSTM) {
+      V o, tc;
+      sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c, splat<VEC>(-2.0f * kLog2e)), o, tc);
+      const V dh_o = mul_(raw_dh[l].get(), o), minus = splat<VEC>(-1.0f), one = splat<VEC>(1.0f);
+      dc[l] = mul_(dh_o, fma_(mul_(tc, minus), tc, one));
+      V d_o = mul_(mul_(dh_o, tc), fma_(o, minus, one));
+      if (!at.whole && !at.valid(l)) dc[l] = d_o = splat<VEC>(0.0f);
+      db[3] = add_(db[3], d_o);
       if (at.whole || (at.ok && at.t0 + l < p.T)) {
         Pack<VEC, BF16> w;
         w.set(d_o);
@@ -651,80 +717,68 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     }
   }
   // what leaves this thread's steps towards earlier ones
-  float E[VEC];
+  V E = d_state(L - 1);
+  E = fma_(n[L - 1], E, E);
+  A = add_(splat<VEC>(1.0f), n[L - 1]);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const float g0 = d_state(L - 1, i);
-    E[i] = fmaf(-u[L - 1][i], g0, g0);
-    A[i] = 1.0f - u[L - 1][i];
-#pragma unroll
-    for (int l = L - 2; l >= 0; --l) {
-      const float g = d_state(l, i) + E[i];
-      E[i] = fmaf(-u[l][i], g, g);
-      A[i] = fmaf(-u[l][i], A[i], A[i]);
-    }
+  for (int l = L - 2; l >= 0; --l) {
+    const V g = add_(d_state(l), E);
+    E = fma_(n[l], g, g);
+    A = fma_(n[l], A, A);
   }
   join_spans<VEC, true>(at.span, A, E, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
   lin_join<CW, NW, true>(p, at.row, kr, p.d_last, s, got, [&](long long state, int, float, float end) {
     if (at.k == 0 && p.d_initial != nullptr) p.d_initial[state] = end;
   });
-  float e[VEC];
-  if (at.ok) {
-    ld_vec<VEC>(&s.start[at.warp][at.chl], e);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) E[i] = fmaf(A[i], e[i], E[i]);
+  E = fma_(A, at.ok ? load_<VEC>(&s.start[at.warp][at.chl]) : splat<VEC>(0.0f), E);
+  to += (L - 1) * G * row_bytes;
 #pragma unroll
   for (int l = L - 1; l >= 0; --l) {
-    constexpr int kHere = G == 4 ? 3 : G;  // gates whose gradients are stored here
-    float d[kHere][VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float g = d_state(l, i) + E[i], q = fmaf(-u[l][i], u[l][i], u[l][i]);  // u (1 - u)
-      E[i] = fmaf(-u[l][i], g, g);
-      if constexpr (G == 4) {
-        const float gi = g * si[l][i];
-        d[0][i] = gi * tz[l][i] * (1.0f - si[l][i]);
-        d[1][i] = g * prev[l][i] * q;
-        d[2][i] = gi * fmaf(-tz[l][i], tz[l][i], 1.0f);
-      } else {
-        d[0][i] = g * (prev[l][i] - (raw[l][1].get(i) + bias[1][i])) * q;
-        d[1][i] = g * u[l][i];
-      }
+    constexpr int kHere = LSTM ? 3 : G;  // gates whose gradients are stored here
+    V d[kHere];
+    const V g = add_(d_state(l), E), minus = splat<VEC>(-1.0f);
+    const V q = fma_(n[l], n[l], n[l]);  // -u (1 - u)
+    E = fma_(n[l], g, g);
+    if constexpr (LSTM) {
+      const V gi = mul_(g, si[l]), one = splat<VEC>(1.0f);
+      d[0] = mul_(mul_(gi, tz[l]), fma_(si[l], minus, one));
+      d[1] = mul_(mul_(g, prev[l]), mul_(q, minus));
+      d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
+    } else {
+      const V mz = scaled<CELL>(raw[l][1], bias[1], 1), mg = mul_(g, minus);  // -z, -g
+      d[0] = mul_(mul_(mg, q), add_(prev[l], mz));
+      d[1] = mul_(mg, n[l]);
     }
-    if (!at.whole) {
+    if (!at.whole && !at.valid(l)) {
 #pragma unroll
-      for (int g = 0; g < kHere; ++g)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) d[g][i] = at.valid(l) ? d[g][i] : 0.0f;
+      for (int j = 0; j < kHere; ++j) d[j] = splat<VEC>(0.0f);
     }
 #pragma unroll
-    for (int g = 0; g < kHere; ++g)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) db[g][i] += d[g][i];
+    for (int j = 0; j < kHere; ++j) db[j] = add_(db[j], d[j]);
     if (at.whole || (at.ok && at.t0 + l < p.T)) {
 #pragma unroll
-      for (int g = 0; g < kHere; ++g) {
+      for (int j = 0; j < kHere; ++j) {
         Pack<VEC, BF16> w;
-        w.set(d[g]);
-        w.store(to + (l * G + g) * row_bytes);
+        w.set(d[j]);
+        w.store(to + j * row_bytes);
       }
     }
+    to -= G * row_bytes;
   }
 #pragma unroll
   for (int o = W::kRow; o < 32; o *= 2) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g) {
+      V other;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) db[g][i] += __shfl_xor_sync(0xffffffffu, db[g][i], o);
+      for (int i = 0; i < VEC; ++i) other[i] = __shfl_xor_sync(0xffffffffu, db[g][i], o);
+      db[g] = add_(db[g], other);
+    }
   }
   if (at.span == 0) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) st_vec<VEC>(&s_db[at.warp][g][at.chl], db[g]);
+    for (int g = 0; g < G; ++g) st_f32_vec<VEC>(&s_db[at.warp][g][at.chl], db[g].v);
   }
   __syncthreads();
   for (int j = tid; j < G * CW; j += blockDim.x) {
@@ -734,6 +788,212 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     for (int w = 0; w < nw; ++w) sum += s_db[w][g][cc];
     p.db_part[((static_cast<long long>(at.b) * p.n_tiles + at.k) * G + g) * p.ND + at.c0 + cc] = sum;
   }
+}
+
+// Many channels: there is no need to cut time. A thread walks its two channels (one, where ND is odd) through the whole sequence, the
+// next steps' loads in flight while it computes; no exchange, a third of the instructions of a tile. The states it keeps for the
+// backward pass are kWalkSteps apart: what the backward walk recomputes between two of them stays in registers.
+constexpr int kWalkSteps = 8, kWalkThreads = 64;
+constexpr long long kWalkChannels = 65536, kWalkOddChannels = 32768;
+
+template <int CELL, int VEC, bool BF16>
+struct Walk {
+  static constexpr int G = LinCell<CELL>::G, S = kWalkSteps;
+  using V = Vec<VEC>;
+  using P = Pack<VEC, BF16>;
+  int b, ch, len;
+  size_t gate;  // bytes from one gate (or hidden state) to the next
+  bool ok;
+  __device__ __forceinline__ Walk(const LinParams& p) {
+    const int per_row = (p.ND + VEC - 1) / VEC;
+    const long long id = static_cast<long long>(blockIdx.x) * kWalkThreads + threadIdx.x;
+    b = static_cast<int>(id / per_row);
+    ch = static_cast<int>(id - static_cast<long long>(b) * per_row) * VEC;
+    ok = b < p.B;
+    gate = static_cast<size_t>(p.ND) * (BF16 ? 2 : 4);
+    len = !ok ? 0 : p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
+  }
+  // `per` values of S steps from step t, those in front of the end of the sequence
+  template <int PER>
+  __device__ __forceinline__ void load(P (&r)[S][PER], const void* base, int T, int t) const {
+    const uint8_t* from = static_cast<const uint8_t*>(base) + (static_cast<size_t>(b) * T + t) * PER * gate + static_cast<size_t>(ch) * (BF16 ? 2 : 4);
+    if (t >= 0 && t <= len - S) {
+#pragma unroll
+      for (int l = 0; l < S; ++l)
+#pragma unroll
+        for (int g = 0; g < PER; ++g) r[l][g].load(from + (l * PER + g) * gate);
+    } else {
+#pragma unroll
+      for (int l = 0; l < S; ++l)
+#pragma unroll
+        for (int g = 0; g < PER; ++g)
+          if (t >= 0 && t < len - l) r[l][g].load(from + (l * PER + g) * gate);
+          else r[l][g].clear();
+    }
+  }
+};
+
+template <int CELL, int VEC, bool BF16>
+__global__ void __launch_bounds__(kWalkThreads, CELL == FRNN_LINEAR_LSTM ? 1 : 7) linear_fwd_walk_kernel(const LinParams p) {
+  using W = Walk<CELL, VEC, BF16>;
+  using Cell = LinCell<CELL>;
+  using V = Vec<VEC>;
+  constexpr int G = W::G, S = W::S;
+  const W w(p);
+  if (!w.ok) return;
+  V bias[G];
+  load_bias<CELL, VEC>(p, true, w.ch, bias);
+  const size_t state = static_cast<size_t>(w.b) * p.ND + w.ch;
+  V c = p.initial != nullptr ? load_<VEC>(p.initial + state) : splat<VEC>(0.0f);
+  const int last_kept = (p.T - 1) / S;  // states 1 .. last_kept are kept, each in front of its step
+  auto steps = [&](const Pack<VEC, BF16> (&raw)[S][G], int t) {
+    if (t > 0 && p.starts != nullptr) st_f32_vec<VEC>(p.starts + (static_cast<size_t>(w.b) * last_kept + t / S - 1) * p.ND + w.ch, c.v);
+    uint8_t* to = static_cast<uint8_t*>(p.hidden) + (static_cast<size_t>(w.b) * p.T + t) * w.gate + static_cast<size_t>(w.ch) * (BF16 ? 2 : 4);
+    V n[S], v[S];
+#pragma unroll
+    for (int l = 0; l < S; ++l) {
+      V x[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
+      Cell::gates(x, n[l], v[l]);
+    }
+#pragma unroll
+    for (int l = 0; l < S; ++l) {
+      if (t + l < w.len) {
+        c = lin_step(n[l], v[l], c);
+        V out = c;
+        if constexpr (CELL == FRNN_LINEAR_LSTM)
+          out = sigmoid_times_tanh(scaled<CELL>(raw[l][G - 1], bias[G - 1], G - 1), mul_(c, splat<VEC>(-2.0f * kLog2e)));
+        Pack<VEC, BF16> o;
+        o.set(out);
+        o.store(to + l * w.gate);
+      }
+    }
+  };
+  // groups of steps on their way: two of the leaky cell, one of the LSTM, whose four gates leave no room for more
+  constexpr int AHEAD = CELL == FRNN_LINEAR_LSTM ? 1 : 2, R = AHEAD + 1;
+  Pack<VEC, BF16> ring[R][S][G];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) w.load(ring[i], p.wx, p.T, i * S);
+  for (int t = 0; t < w.len; t += R * S) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i > 0 && t + i * S >= w.len) break;
+      w.load(ring[(i + AHEAD) % R], p.wx, p.T, t + (i + AHEAD) * S);
+      steps(ring[i], t + i * S);
+    }
+  }
+  st_f32_vec<VEC>(p.last + state, c.v);
+  Pack<VEC, BF16> zero;
+  zero.clear();
+  for (int q = w.len; q < p.T; ++q)
+    zero.store(static_cast<uint8_t*>(p.hidden) + (static_cast<size_t>(w.b) * p.T + q) * w.gate + static_cast<size_t>(w.ch) * (BF16 ? 2 : 4));
+}
+
+template <int CELL, int VEC, bool BF16>
+__global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const LinParams p) {
+  using W = Walk<CELL, VEC, BF16>;
+  using Cell = LinCell<CELL>;
+  using V = Vec<VEC>;
+  constexpr bool LSTM = CELL == FRNN_LINEAR_LSTM;
+  constexpr int G = W::G, S = W::S;
+  const W w(p);
+  if (!w.ok) return;
+  V bias[G], db[G];
+  load_bias<CELL, VEC>(p, true, w.ch, bias);
+#pragma unroll
+  for (int g = 0; g < G; ++g) db[g] = splat<VEC>(0.0f);
+  const size_t state = static_cast<size_t>(w.b) * p.ND + w.ch;
+  const int last_kept = (p.T - 1) / S;
+  uint8_t* const to = static_cast<uint8_t*>(p.d_wx) + static_cast<size_t>(w.b) * p.T * G * w.gate + static_cast<size_t>(w.ch) * (BF16 ? 2 : 4);
+  Pack<VEC, BF16> zero;
+  zero.clear();
+  for (int q = w.len; q < p.T; ++q)
+#pragma unroll
+    for (int g = 0; g < G; ++g) zero.store(to + (static_cast<size_t>(q) * G + g) * w.gate);
+  auto start = [&](int t) {
+    if (t < 0) return splat<VEC>(0.0f);
+    if (t > 0) return load_<VEC>(p.starts + (static_cast<size_t>(w.b) * last_kept + t / S - 1) * p.ND + w.ch);
+    return p.initial != nullptr ? load_<VEC>(p.initial + state) : splat<VEC>(0.0f);
+  };
+  V E = p.d_last != nullptr ? load_<VEC>(p.d_last + state) : splat<VEC>(0.0f);
+  const V minus = splat<VEC>(-1.0f), one = splat<VEC>(1.0f);
+  auto steps = [&](const Pack<VEC, BF16> (&raw)[S][G], const Pack<VEC, BF16> (&dh)[S][1], V c, int t) {
+    V n[S], prev[S], si[LSTM ? S : 1], tz[LSTM ? S : 1], sum[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) sum[g] = splat<VEC>(0.0f);
+#pragma unroll
+    for (int l = 0; l < S; ++l) {
+      V x[G], v;
+#pragma unroll
+      for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
+      if constexpr (LSTM) {
+        n[l] = rcp_(fma_(exp2_(x[1]), minus, minus));
+        sigmoid_tanh(x[0], x[2], si[l], tz[l]);
+        v = mul_(si[l], tz[l]);
+      } else {
+        Cell::gates(x, n[l], v);
+      }
+      prev[l] = c;
+      c = lin_step(n[l], v, c);
+    }
+#pragma unroll
+    for (int l = S - 1; l >= 0; --l) {
+      if (t + l < w.len) {
+        V d[G], g = dh[l][0].get();
+        const V q = fma_(n[l], n[l], n[l]);  // -u (1 - u)
+        if constexpr (LSTM) {
+          V o, tc;
+          const V c_l = l == S - 1 ? c : prev[l == S - 1 ? l : l + 1];
+          sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c_l, splat<VEC>(-2.0f * kLog2e)), o, tc);
+          const V dh_o = mul_(g, o);
+          d[3] = mul_(mul_(dh_o, tc), fma_(o, minus, one));
+          g = fma_(dh_o, fma_(mul_(tc, minus), tc, one), E);
+          const V gi = mul_(g, si[l]);
+          d[0] = mul_(mul_(gi, tz[l]), fma_(si[l], minus, one));
+          d[1] = mul_(mul_(g, prev[l]), mul_(q, minus));
+          d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
+        } else {
+          g = add_(g, E);
+          const V mz = scaled<CELL>(raw[l][1], bias[1], 1), mg = mul_(g, minus);  // -z, -g
+          d[0] = mul_(mul_(mg, q), add_(prev[l], mz));
+          d[1] = mul_(mg, n[l]);
+        }
+        E = fma_(n[l], g, g);
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          sum[j] = add_(sum[j], d[j]);
+          Pack<VEC, BF16> o;
+          o.set(d[j]);
+          o.store(to + (static_cast<size_t>(t + l) * G + j) * w.gate);
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) db[g] = add_(db[g], sum[g]);
+  };
+  Pack<VEC, BF16> raw[2][S][G], dh[2][S][1];
+  V c[2];
+  int t = (w.len - 1) / S * S;
+  if (w.len > 0) {
+    w.load(raw[0], p.wx, p.T, t);
+    w.load(dh[0], p.d_hidden, p.T, t);
+    c[0] = start(t);
+  }
+  for (; t >= 0 && w.len > 0; t -= 2 * S) {
+    w.load(raw[1], p.wx, p.T, t - S);
+    w.load(dh[1], p.d_hidden, p.T, t - S);
+    c[1] = start(t - S);
+    steps(raw[0], dh[0], c[0], t);
+    if (t - S < 0) break;
+    w.load(raw[0], p.wx, p.T, t - 2 * S);
+    w.load(dh[0], p.d_hidden, p.T, t - 2 * S);
+    c[0] = start(t - 2 * S);
+    steps(raw[1], dh[1], c[1], t - S);
+  }
+  if (p.d_initial != nullptr) st_f32_vec<VEC>(p.d_initial + state, E.v);
+#pragma unroll
+  for (int g = 0; g < G; ++g) st_f32_vec<VEC>(p.db_part + (static_cast<size_t>(w.b) * G + g) * p.ND + w.ch, db[g].v);
 }
 
 // out[j] = sum over rows of part[row][j], in a fixed order: 32 columns to a block, its 32 warps take rows in turn.
@@ -753,6 +1013,17 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
 
 int lin_vec(int ND) { return ND % 4 == 0 ? 4 : 1; }
 int lin_channels(int ND) { return lin_vec(ND) == 1 ? 32 : 64; }
+// Enough channels for every SM to keep its loads in flight without cutting time.
+bool lin_walk(long long B, long long ND) { return B * ND >= (ND % 4 == 0 ? kWalkChannels : kWalkOddChannels); }
+
+template <int CELL, int VEC, bool BF16, bool BACKWARD>
+int launch_walk(const LinParams& p, cudaStream_t s) {
+  const long long threads = static_cast<long long>(p.B) * ((p.ND + VEC - 1) / VEC), blocks = (threads + kWalkThreads - 1) / kWalkThreads;
+  if (blocks > 0x7fffffffLL) return -2;
+  if constexpr (BACKWARD) linear_bwd_walk_kernel<CELL, VEC, BF16><<<static_cast<unsigned>(blocks), kWalkThreads, 0, s>>>(p);
+  else linear_fwd_walk_kernel<CELL, VEC, BF16><<<static_cast<unsigned>(blocks), kWalkThreads, 0, s>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
 
 template <int CELL, int VEC, int LF, int LB, bool BF16>
 int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
@@ -762,7 +1033,8 @@ int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
   const int l = backward ? LB : LF;
   int warps = backward ? kNWB : kNWF;
   if (p.n_tiles == 1) warps = (p.T + kSpans * l - 1) / (kSpans * l);
-  if (!backward) linear_fwd_kernel<CELL, VEC, LF, kNWF, 512 / (kNWF * 32), BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
+  constexpr int kCtas = CELL == FRNN_LINEAR_LEAKY && BF16 ? 3 : 512 / (kNWF * 32);
+  if (!backward) linear_fwd_kernel<CELL, VEC, LF, kNWF, kCtas, BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
   else linear_bwd_kernel<CELL, VEC, LB, kNWB, 512 / (kNWB * 32), BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
@@ -771,6 +1043,11 @@ int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
 template <int CELL, bool BF16>
 int launch_vec(const LinParams& p, bool backward, cudaStream_t s) {
   constexpr bool kLstm = CELL == FRNN_LINEAR_LSTM;
+  if (lin_walk(p.B, p.ND)) {
+    constexpr int kBack = kLstm ? 1 : 2;  // two channels of the LSTM's backward walk do not fit the registers
+    if (backward) return p.ND % 2 == 0 ? launch_walk<CELL, kBack, BF16, true>(p, s) : launch_walk<CELL, 1, BF16, true>(p, s);
+    return p.ND % 2 == 0 ? launch_walk<CELL, 2, BF16, false>(p, s) : launch_walk<CELL, 1, BF16, false>(p, s);
+  }
   if (lin_vec(p.ND) == 4) return launch_one<CELL, 4, 8, kLstm ? 4 : 8, BF16>(p, backward, s);
   return launch_one<CELL, 1, 16, kLstm ? 8 : 16, BF16>(p, backward, s);
 }
@@ -813,6 +1090,14 @@ extern "C" int frnn_b200_linear_plan(int function, int B, int T, int N, int D, f
   if (blocks * tiles > 0x7fffffffLL) return -2;
   *out = {};
   out->gates = gates;
+  if (lin_walk(B, nd)) {
+    out->tile_steps = kWalkSteps;
+    out->tile_channels = nd % 2 == 0 ? 2 : 1;
+    out->tiles = 1;
+    out->starts_bytes = 4 * B * ((T - 1) / kWalkSteps) * nd;
+    if (B > 1) out->dbpart_bytes = 4LL * B * gates * nd;
+    return 0;
+  }
   out->tile_steps = steps;
   out->tile_channels = channels;
   out->tiles = static_cast<int>(tiles);

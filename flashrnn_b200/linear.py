@@ -35,10 +35,10 @@ def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Option
     if last is None:
         last = torch.empty((1, B, 1, N, D), dtype=torch.float32, device=dev)
     starts = exchange = err = None
+    if keep and plan.starts_bytes:
+        starts = torch.empty(plan.starts_bytes // 4, dtype=torch.float32, device=dev)
     if plan.exchange_bytes:   # several tiles, which wait for one another
         exchange, err = torch.empty(plan.exchange_bytes, dtype=torch.uint8, device=dev), _error_word(dev)
-        if keep:
-            starts = torch.empty(plan.starts_bytes // 4, dtype=torch.float32, device=dev)
     rc = lib.frnn_b200_linear_forward(
         _lib.LINEAR_CELLS[function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
         hidden.data_ptr(), last.data_ptr(), _ptr(starts), _ptr(exchange), B, T, N, D, 0, _ptr(err), _stream(dev))

@@ -225,11 +225,11 @@ enum { FRNN_LINEAR_LEAKY = 0, FRNN_LINEAR_LSTM = 1 };
 
 typedef struct frnn_b200_linear_plan {
   int gates;
-  int tile_steps, tile_channels;  /* of one CTA                                                             */
-  int tiles;                      /* along time                                                             */
+  int tile_steps, tile_channels;  /* of one CTA; of one thread that walks the whole sequence (many channels) */
+  int tiles;                      /* along time that wait for one another; 1: none                          */
   int64_t exchange_bytes;         /* scratch of either call, 16-byte aligned; 0: exchange and err may be NULL */
-  int64_t starts_bytes;           /* fp32 [B][tiles - 1][N][D], forward -> backward                         */
-  int64_t dbpart_bytes;           /* fp32 [B * tiles][G][N][D], scratch of the backward call                */
+  int64_t starts_bytes;           /* fp32 states every tile_steps steps, forward -> backward                */
+  int64_t dbpart_bytes;           /* fp32 [B * tiles][G][N][D], scratch of the backward call; 0: not needed */
 } frnn_b200_linear_plan_t;
 
 int frnn_b200_linear_plan(int function, int B, int T, int N, int D, frnn_b200_linear_plan_t* out);

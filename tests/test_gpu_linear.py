@@ -60,6 +60,23 @@ def test_values_and_gradients(function, dtype, shape, cuda_device):
     L.check(got, ref, L.bounds(ref, wx, b, s, T, dh, dl))
 
 
+# so many channels that a thread walks the whole sequence: even and odd widths, lengths around the 8 and 16 steps that it has on
+# their way
+@pytest.mark.parametrize("shape", [(512, 1, 1, 128), (512, 7, 2, 64), (512, 8, 1, 128), (256, 9, 2, 129), (200, 17, 1, 330), (410, 41, 5, 33),
+                                   (1100, 25, 1, 30)], ids=str)
+@pytest.mark.parametrize("dtype", [B16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("function", ["leaky", "lstm"])
+def test_many_channels(function, dtype, shape, cuda_device):
+    from flashrnn_b200 import _lib
+
+    B, T, N, D = shape
+    assert _lib.linear_plan(function, *shape).exchange_bytes == 0 and _lib.linear_plan(function, *shape).tile_steps == 8
+    wx, b, s, n, dh, dl = make(function, *shape, dtype, T + D, cuda_device, states=T % 3 > 0, lengths="ragged" if T % 2 else None)
+    got = step(function, wx, b, s, n, dh, dl)
+    ref = L.run_reference(wx, b, s, function, n, dh, dl)
+    L.check(got, ref, L.bounds(ref, wx, b, s, T, dh, dl))
+
+
 @pytest.mark.parametrize("function", ["leaky", "lstm"])
 @pytest.mark.parametrize("T", [7, 130, 2100])
 def test_padding_is_never_read(function, T, cuda_device):
@@ -135,9 +152,10 @@ def test_it_is_the_lstm_without_its_recurrent_matrix(cuda_device):
 
 
 @pytest.mark.parametrize("T", [1, 100, 700, 3000])
+@pytest.mark.parametrize("B", [6, 400])
 @pytest.mark.parametrize("function", ["leaky", "lstm"])
-def test_same_bits_every_time(function, T, cuda_device):
-    wx, b, s, n, dh, dl = make(function, 6, T, 3, 100, B16, 6, cuda_device, lengths="ragged")
+def test_same_bits_every_time(function, B, T, cuda_device):
+    wx, b, s, n, dh, dl = make(function, B, min(T, 100000 // B), 3, 100, B16, 6, cuda_device, lengths="ragged")
     first = step(function, wx, b, s, n, dh, dl)
     for _ in range(5):
         again = step(function, wx, b, s, n, dh, dl)
