@@ -85,7 +85,7 @@ class LinearPlan(ctypes.Structure):
 class ProductPlan(ctypes.Structure):
     """Mirror of ``frnn_b200_product_plan_t``."""
 
-    _fields_ = [("forward_work_bytes", c_int64), ("backward_work_bytes", c_int64), ("dbpart_bytes", c_int64)]
+    _fields_ = [("forward_work_bytes", c_int64), ("backward_work_bytes", c_int64), ("dbpart_bytes", c_int64), ("forward_waits", c_int)]
 
 
 # name -> (restype, argtypes); must list every function declared in include/flashrnn_b200.h

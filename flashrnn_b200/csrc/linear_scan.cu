@@ -379,37 +379,31 @@ struct Shared {
 // (null: zeros) is what the row starts from; done(state, channel, carry, end) is called per channel with its place in [B][ND], what
 // the tile starts from and what it ends with. The maps are in place and a barrier is behind them.
 template <int CW, int NW, bool REVERSE, typename F>
-__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, const float* first, Shared<CW, NW>& s, const Fetched<CW, NW>& got,
+__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, const float* first, Shared<CW, NW>& s, Fetched<CW, NW>& got,
                                          F done) {
   const int nw = blockDim.x >> 5, b = row / p.n_cg, c0 = (row % p.n_cg) * CW, n_channels = min(CW, p.ND - c0);
   const Exchange x(p, row, CW);
-  float a[CW / 32], h[CW / 32];
-#pragma unroll
-  for (int r = 0; r < CW / 32; ++r) {  // a second round only in a CTA of one warp
-    const int c = threadIdx.x + r * blockDim.x;
-    a[r] = 1.0f; h[r] = 0.0f;
-    if (c >= n_channels) continue;
+  const int c = threadIdx.x;  // a CTA has as many threads as a tile has channels, or more
+  float a = 1.0f, h = 0.0f;
+  if (c < n_channels) {
 #pragma unroll 4
     for (int i = 0; i < nw; ++i) {
       const int w = REVERSE ? nw - 1 - i : i;
       const float wa = s.a[w][c], wh = s.h[w][c];
-      h[r] = fmaf(wa, h[r], wh);
-      a[r] *= wa;
+      h = fmaf(wa, h, wh);
+      a *= wa;
     }
-    if (p.n_tiles > 1) lin_publish(p, x, k, c, CW, a[r], h[r]);
+    if (p.n_tiles > 1) lin_publish(p, x, k, c, CW, a, h);
   }
   if (p.n_tiles > 1) {
-    const_cast<Fetched<CW, NW>&>(got).put(p, s.prev);
+    got.put(p, s.prev);
     __syncthreads();
   }
-#pragma unroll
-  for (int r = 0; r < CW / 32; ++r) {
-    const int c = threadIdx.x + r * blockDim.x;
-    if (c >= n_channels) continue;
+  if (c < n_channels) {
     const long long state = static_cast<long long>(b) * p.ND + c0 + c;
     float carry = first != nullptr && k < kGroup ? __ldg(first + state) : 0.0f;
-    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, c, s.prev, carry, a[r], h[r]);
-    done(state, c0 + c, carry, fmaf(a[r], carry, h[r]));
+    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, c, s.prev, carry, a, h);
+    done(state, c0 + c, carry, fmaf(a, carry, h));
 #pragma unroll 4
     for (int i = 0; i < nw; ++i) {
       const int w = REVERSE ? nw - 1 - i : i;
@@ -634,14 +628,11 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   Fetched<CW, NW> got;
   if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), kr, min(CW, p.ND - at.c0));
   // the state in front of the tile, channels as in lin_join
-  float before[CW / 32];
-#pragma unroll
-  for (int r = 0; r < CW / 32; ++r) {
-    const int c = tid + r * blockDim.x;
-    before[r] = 0.0f;
-    if (c >= min(CW, p.ND - at.c0)) continue;
-    if (at.k > 0) before[r] = __ldg(p.starts + (static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + at.c0 + c);
-    else if (p.initial != nullptr) before[r] = __ldg(p.initial + static_cast<long long>(at.b) * p.ND + at.c0 + c);
+  const bool mine = tid < min(CW, p.ND - at.c0);
+  float before = 0.0f;
+  if (mine) {
+    if (at.k > 0) before = __ldg(p.starts + (static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + at.c0 + tid);
+    else if (p.initial != nullptr) before = __ldg(p.initial + static_cast<long long>(at.b) * p.ND + at.c0 + tid);
   }
   V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
@@ -674,15 +665,11 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   }
   join_spans<VEC, false>(at.span, A, H, &f_a[at.warp][at.chl], &f_h[at.warp][at.chl]);
   __syncthreads();
-#pragma unroll
-  for (int r = 0; r < CW / 32; ++r) {
-    const int c = tid + r * blockDim.x;
-    if (c >= min(CW, p.ND - at.c0)) continue;
-    float v = before[r];
+  if (mine) {
 #pragma unroll 4
     for (int w = 0; w < nw; ++w) {
-      s.start[w][c] = v;
-      v = fmaf(f_a[w][c], v, f_h[w][c]);
+      s.start[w][tid] = before;
+      before = fmaf(f_a[w][tid], before, f_h[w][tid]);
     }
   }
   __syncthreads();
@@ -1013,8 +1000,8 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
 
 int lin_vec(int ND) { return ND % 4 == 0 ? 4 : 1; }
 int lin_channels(int ND) { return lin_vec(ND) == 1 ? 32 : 64; }
-// Enough channels for every SM to keep its loads in flight without cutting time.
-bool lin_walk(long long B, long long ND) { return B * ND >= (ND % 4 == 0 ? kWalkChannels : kWalkOddChannels); }
+// Enough channels for every SM to keep its loads in flight without cutting time, or next to no time to cut.
+bool lin_walk(long long B, int T, long long ND) { return T <= 2 * kWalkSteps || B * ND >= (ND % 4 == 0 ? kWalkChannels : kWalkOddChannels); }
 
 template <int CELL, int VEC, bool BF16, bool BACKWARD>
 int launch_walk(const LinParams& p, cudaStream_t s) {
@@ -1032,6 +1019,8 @@ int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
   if (tiles > 0x7fffffffLL) return -2;
   const int l = backward ? LB : LF;
   int warps = backward ? kNWB : kNWF;
+  static_assert((2 * kWalkSteps + kSpans * LF) / (kSpans * LF) * 32 >= Lanes<VEC>::kChannels, "a thread for every channel of the shortest tile");
+  static_assert((2 * kWalkSteps + kSpans * LB) / (kSpans * LB) * 32 >= Lanes<VEC>::kChannels, "a thread for every channel of the shortest tile");
   if (p.n_tiles == 1) warps = (p.T + kSpans * l - 1) / (kSpans * l);
   constexpr int kCtas = CELL == FRNN_LINEAR_LEAKY && BF16 ? 3 : 512 / (kNWF * 32);
   if (!backward) linear_fwd_kernel<CELL, VEC, LF, kNWF, kCtas, BF16><<<static_cast<unsigned>(tiles), warps * 32, 0, s>>>(p);
@@ -1043,7 +1032,7 @@ int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
 template <int CELL, bool BF16>
 int launch_vec(const LinParams& p, bool backward, cudaStream_t s) {
   constexpr bool kLstm = CELL == FRNN_LINEAR_LSTM;
-  if (lin_walk(p.B, p.ND)) {
+  if (lin_walk(p.B, p.T, p.ND)) {
     constexpr int kBack = kLstm ? 1 : 2;  // two channels of the LSTM's backward walk do not fit the registers
     if (backward) return p.ND % 2 == 0 ? launch_walk<CELL, kBack, BF16, true>(p, s) : launch_walk<CELL, 1, BF16, true>(p, s);
     return p.ND % 2 == 0 ? launch_walk<CELL, 2, BF16, false>(p, s) : launch_walk<CELL, 1, BF16, false>(p, s);
@@ -1090,7 +1079,7 @@ extern "C" int frnn_b200_linear_plan(int function, int B, int T, int N, int D, f
   if (blocks * tiles > 0x7fffffffLL) return -2;
   *out = {};
   out->gates = gates;
-  if (lin_walk(B, nd)) {
+  if (lin_walk(B, T, nd)) {
     out->tile_steps = kWalkSteps;
     out->tile_channels = nd % 2 == 0 ? 2 : 1;
     out->tiles = 1;

@@ -14,7 +14,8 @@
 // single CTAs with 128 x 256 tiles move 48. Warp 8 feeds the ring by TMA (128-byte swizzle), one thread of the even CTA issues
 // the MMAs of both, 8 warps of each CTA take the accumulator out of tensor memory: two accumulators, so the epilogue of a tile
 // runs under the contraction of the next. Rows and columns past the edges are read as zeros and not stored.
-// Few tiles with a long K are cut along K: partial tiles in fp32, summed in order by product_join_kernel, which then has the epilogue.
+// Tiles that do not fill another round of all pairs are cut along K, so that their parts do: these go out in fp32 and are summed in
+// order by product_join_kernel, which then has the epilogue. Up to 32 rows take product_rows_kernel, which reads W once from registers.
 #include "../../include/flashrnn_b200.h"
 
 #include "frnn_common.cuh"
@@ -40,8 +41,10 @@ struct ProductParams {
   int* err;
   int bias_bf16, act, has_residual, has_z;
   int M, N, K;       // of the contraction
-  int n_mt, n_nt, chunks, chunks_per_split;
-  long long n_tiles;
+  int n_nt, chunks;
+  // units of work: `whole` tiles, then the others in `parts` of chunks_per_part chunks of K each
+  int parts, chunks_per_part;
+  long long whole, n_units;
 };
 
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
@@ -53,11 +56,6 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
                "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1)
-               : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src),
-               "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
 // Both CTAs of the pair take part in these, one warp each.
@@ -198,12 +196,12 @@ __device__ __forceinline__ void add_bf16(const uint32_t (&w)[4], float* v) {
   for (int i = 0; i < 4; ++i) add2(v[2 * i], v[2 * i + 1], bf16_lo(w[i]), bf16_hi(w[i]));
 }
 
-// A_MN / B_MN: the operand's rows in memory run along M / N instead of K. PARTIAL: fp32 tiles of one of several parts of K, no epilogue.
-template <bool A_MN, bool B_MN, int NP, bool PARTIAL, int ACT>
+// A_MN / B_MN: the operand's rows in memory run along M / N instead of K.
+template <bool A_MN, bool B_MN, int NP, int ACT>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
                const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
-               const __grid_constant__ CUtensorMap z_map) {
+               const __grid_constant__ CUtensorMap z_map, const __grid_constant__ CUtensorMap work_map) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int kStages = stages_of(NP, B_MN);
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2], s_done;
@@ -246,16 +244,22 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
   tc_fence_after_sync();
   const uint32_t tbase = s_tmem_base;
 
-  // tile -> rows, columns, part of K
-  struct Tile { int m0, n0, split, c_begin, c_end; };
+  // rows, columns, part of K of a unit; row0: of a part, where its sums go
+  struct Tile { int m0, n0, row0, c_begin, c_end; };
   auto tile_at = [&](long long t) {
     Tile r;
+    r.row0 = -1;
+    r.c_begin = 0;
+    r.c_end = p.chunks;
+    if (t >= p.whole) {
+      const int u = static_cast<int>(t - p.whole), part = u % p.parts;
+      r.row0 = u * 256;
+      r.c_begin = part * p.chunks_per_part;
+      r.c_end = min(r.c_begin + p.chunks_per_part, p.chunks);
+      t = p.whole + u / p.parts;
+    }
     r.n0 = static_cast<int>(t % p.n_nt) * NP;
-    t /= p.n_nt;
-    r.m0 = static_cast<int>(t % p.n_mt) * 256;
-    r.split = static_cast<int>(t / p.n_mt);
-    r.c_begin = r.split * p.chunks_per_split;
-    r.c_end = min(r.c_begin + p.chunks_per_split, p.chunks);
+    r.m0 = static_cast<int>(t / p.n_nt) * 256;
     return r;
   };
 
@@ -263,7 +267,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
     if (lane == 0) {
       uint32_t s = 0, round = 0;
       bool dead = false;
-      for (long long t = pair; t < p.n_tiles && !dead; t += pairs) {
+      for (long long t = pair; t < p.n_units && !dead; t += pairs) {
         const Tile tile = tile_at(t);
         const int ma = tile.m0 + 128 * cta, nb = tile.n0 + NH * cta;
         for (int i = tile.c_begin; i < tile.c_end; ++i) {
@@ -308,7 +312,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       const uint32_t idesc = umma_idesc_bf16(256, NP, A_MN, B_MN);
       uint32_t s = 0, round = 0, li = 0;
       bool dead = false;
-      for (long long t = pair; t < p.n_tiles && !dead; t += pairs, ++li) {
+      for (long long t = pair; t < p.n_units && !dead; t += pairs, ++li) {
         const Tile tile = tile_at(t);
         const uint32_t a = li & 1u;
         if (li >= 2 && !mbar_wait_bounded<true, true>(smem_u32(&s_acc_empty[a]), ((li >> 1) - 1) & 1, kLimit, abort_flag)) {
@@ -345,35 +349,33 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
     }
   } else {
     const int q = warp & 3, half = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; columns
-    constexpr int CW = PARTIAL ? 32 : 64;      // columns of a piece: 128 bytes
-    constexpr int kPieces = NP / CW;           // of the tile, in turn to the two warps of a quarter
+    constexpr int CW = 64;            // columns of a piece: 128 bytes
+    constexpr int kPieces = NP / CW;  // of the tile, in turn to the two warps of a quarter
     const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 2u * kBufBytes;
     const uint32_t my_row = static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
     // Without z the pieces take the two buffers in turn; with it z goes through the first, y through the second. The residual's
     // piece is loaded into the buffer that y leaves from.
-    const bool z_too = !PARTIAL && ACT != FRNN_ACT_NONE && p.has_z;
+    const bool z_too = ACT != FRNN_ACT_NONE && p.has_z;
     uint32_t li = 0, used = 0, res_phase = 0;  // used: pieces staged so far; res_phase: a bit per buffer
     auto ask_residual = [&](uint32_t bi, int j, int m) {
       const uint32_t bar = smem_u32(&s_res[warp][bi]);
       mbar_arrive_expect_tx(bar, kBufBytes);
       tma_load_2d(buf0 + bi * kBufBytes, &res_map, bar, j, m);
     };
-    for (long long t = pair; t < p.n_tiles; t += pairs, ++li) {
+    for (long long t = pair; t < p.n_units; t += pairs, ++li) {
       const Tile tile = tile_at(t);
       const uint32_t a = li & 1u;
       const int mw = tile.m0 + 128 * cta + 32 * q, j0 = tile.n0;
-      const bool any = mw < p.M;   // warp-uniform
-      if constexpr (!PARTIAL) {
-        if (p.has_residual && any && lane == 0) {  // while the tensor cores work
-          tma_store_wait_read<0>();
-          if (z_too) {
-            if (j0 + half * CW < p.N) ask_residual(1, j0 + half * CW, mw);
-          } else {
+      const bool any = mw < p.M, part = tile.row0 >= 0;  // warp-uniform
+      if (p.has_residual && any && !part && lane == 0) {   // while the tensor cores work
+        tma_store_wait_read<0>();
+        if (z_too) {
+          if (j0 + half * CW < p.N) ask_residual(1, j0 + half * CW, mw);
+        } else {
 #pragma unroll
-            for (int i = 0; i < kPieces / 2 + kPieces % 2; ++i) {
-              const int piece = half + 2 * i;
-              if (piece < kPieces && j0 + piece * CW < p.N) ask_residual((used + i) & 1u, j0 + piece * CW, mw);
-            }
+          for (int i = 0; i < kPieces / 2 + kPieces % 2; ++i) {
+            const int piece = half + 2 * i;
+            if (piece < kPieces && j0 + piece * CW < p.N) ask_residual((used + i) & 1u, j0 + piece * CW, mw);
           }
         }
       }
@@ -383,80 +385,92 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         break;
       }
       tc_fence_after_sync();
+      auto release = [&]() {  // the accumulator is in registers: the next unit but one may have it
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s_acc_empty[a]), 0));
+      };
+      if (part) {
+        constexpr int kParts = NP / 32;  // pieces of 32 columns in fp32
+        if (lane == 0) tma_store_wait_read<0>();
+#pragma unroll 1
+        for (int i = half; i < kParts; i += 2) {
+          uint32_t v[32];
+          tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * 32), v);
+          tmem_ld_wait();
+          if (i + 2 >= kParts) release();
+          const uint32_t buf = buf0 + (used & 1u) * kBufBytes + my_row;
+          ++used;
+          if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t w[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+            st_shared_v4(buf + ((k ^ sw) << 4), w);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&work_map, buf, i * 32, tile.row0 + 128 * cta + 32 * q);
+            tma_store_commit();
+          }
+        }
+        continue;
+      }
 #pragma unroll 1
       for (int i = half; i < kPieces; i += 2) {
         const int c = a * NP + i * CW, j = j0 + i * CW;
         float v[CW];
         tmem_ld_x32(tmem_addr(tbase, 32 * q, c), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        if constexpr (CW == 64) tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
-        if (i + 2 >= kPieces) {  // the accumulator is in registers: the next tile but one may have it
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s_acc_empty[a]), 0));
-        }
+        if (i + 2 >= kPieces) release();
         if (!any || j >= p.N) continue;
         const uint32_t bi = z_too ? 1u : used & 1u, buf = buf0 + bi * kBufBytes + my_row;
         ++used;
-        if constexpr (PARTIAL) {
-          if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
-          __syncwarp();
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
+        }
+        if (lane == 0) {
+          if (z_too) tma_store_wait_read<0>();
+          else if (!p.has_residual) tma_store_wait_read<1>();
+        }
+        __syncwarp();
+        if (z_too) {
+          if (p.has_residual && i >= 2 && lane == 0) ask_residual(1, j, mw);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const uint32_t w[4] = {__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])};
-            st_shared_v4(buf + ((k ^ sw) << 4), w);
+            uint32_t w[4];
+            keep_slope<ACT>(&v[8 * k], w);
+            st_shared_v4(buf0 + my_row + ((k ^ sw) << 4), w);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_3d(&out_map, buf, j, mw, tile.split);
-            tma_store_commit();
+        }
+        act_row<ACT>(v);
+        if (p.has_residual) {
+          if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][bi]), (res_phase >> bi) & 1u, kLimit, abort_flag)) {
+            if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
           }
-        } else {
-          if (p.bias != nullptr) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
-          }
-          if (lane == 0) {
-            if (z_too) tma_store_wait_read<0>();
-            else if (!p.has_residual) tma_store_wait_read<1>();
-          }
-          __syncwarp();
-          if (z_too) {
-            if (p.has_residual && i >= 2 && lane == 0) ask_residual(1, j, mw);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              uint32_t w[4];
-              keep_slope<ACT>(&v[8 * k], w);
-              st_shared_v4(buf0 + my_row + ((k ^ sw) << 4), w);
-            }
-          }
-          act_row<ACT>(v);
-          if (p.has_residual) {
-            if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][bi]), (res_phase >> bi) & 1u, kLimit, abort_flag)) {
-              if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
-            }
-            res_phase ^= 1u << bi;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              uint32_t w[4];
-              ld_shared_v4(buf + ((k ^ sw) << 4), w);
-              add_bf16(w, &v[8 * k]);
-            }
-          }
+          res_phase ^= 1u << bi;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float* f = &v[8 * k];
-            const uint32_t w[4] = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
-            st_shared_v4(buf + ((k ^ sw) << 4), w);
+            uint32_t w[4];
+            ld_shared_v4(buf + ((k ^ sw) << 4), w);
+            add_bf16(w, &v[8 * k]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&out_map, buf, j, mw);
-            if (z_too) tma_store_2d(&z_map, buf0, j, mw);
-            tma_store_commit();
-          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float* f = &v[8 * k];
+          const uint32_t w[4] = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+          st_shared_v4(buf + ((k ^ sw) << 4), w);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&out_map, buf, j, mw);
+          if (z_too) tma_store_2d(&z_map, buf0, j, mw);
+          tma_store_commit();
         }
       }
     }
@@ -468,23 +482,28 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
   if (warp == 9) tmem_dealloc_pair(tbase, kCols);
 }
 
-// out = epilogue(sum over parts of work), eight columns of a row to a thread.
+// out = epilogue(sum over the parts of a tile), eight columns of a row to a thread; work [tile][part][256][np].
 template <int ACT>
-__global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p, const float* __restrict__ work, int parts,
+__global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p, const float* __restrict__ work, int np,
                                                            const __nv_bfloat16* __restrict__ residual, __nv_bfloat16* __restrict__ out,
                                                            uint4* __restrict__ z) {
-  const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 8, n = static_cast<long long>(p.M) * p.N;
-  if (i >= n) return;
+  const int per_row = np / 8, blocks = per_row, tile = blockIdx.x / blocks, at = (blockIdx.x % blocks) * 256 + threadIdx.x;  // 256 rows
+  const int row = at / per_row, col = at % per_row * 8;
+  const long long t = p.whole + tile;
+  const int m = static_cast<int>(t / p.n_nt) * 256 + row, j = static_cast<int>(t % p.n_nt) * np + col;
+  if (m >= p.M || j >= p.N) return;
+  const float* from = work + (static_cast<long long>(tile) * p.parts * 256 + row) * np + col;
   float v[8];
-  ld_f32_vec<8>(work + i, v);
+  ld_f32_vec<8>(from, v);
 #pragma unroll 4
-  for (int s = 1; s < parts; ++s) {
+  for (int s = 1; s < p.parts; ++s) {
     float w[8];
-    ld_f32_vec<8>(work + s * n + i, w);
+    ld_f32_vec<8>(from + static_cast<long long>(s) * 256 * np, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += w[e];
   }
-  if (p.bias != nullptr) add_bias(p, static_cast<int>(i % p.N), v);
+  if (p.bias != nullptr) add_bias(p, j, v);
+  const long long i = static_cast<long long>(m) * p.N + j;
   if (z != nullptr) {
     uint32_t w[4];
     keep_slope<ACT>(v, w);
@@ -499,37 +518,118 @@ __global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p
   *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// Up to 32 rows: W is read once, from where it lies into the registers of mma.sync (16 outputs x 16 k's), the rows of x are the other
+// operand, eight to an instruction. The tensor pipe's rate does not matter here, the time to get W does: a warp has an eighth of K and
+// all of its loads in flight. The order of k's inside a product is free as long as both operands have the same: a lane takes 16 bytes, eight
+// neighbouring k's, which are two instructions' fragments.
+constexpr int kRowsMax = 32, kRowsWarps = 8;
+template <int ACT, int NB>
+__global__ void __launch_bounds__(kRowsWarps * 32) product_rows_kernel(const ProductParams p, const __nv_bfloat16* __restrict__ x,
+                                                                     const __nv_bfloat16* __restrict__ w,
+                                                                     const __nv_bfloat16* __restrict__ residual,
+                                                                     __nv_bfloat16* __restrict__ out, __half* __restrict__ z) {
+  __shared__ float s_sum[kRowsWarps][NB * 8][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, j0 = blockIdx.x * 16;
+  float d[NB][4];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[n][e] = 0.0f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const bool lo = j0 + g < p.N, hi = j0 + g + 8 < p.N;
+  const __nv_bfloat16 *w0 = w + static_cast<size_t>(j0 + g) * p.K, *w1 = w0 + static_cast<size_t>(8) * p.K;
+#pragma unroll 4
+  for (int kb = warp * 32; kb < p.K; kb += kRowsWarps * 32) {
+    const int k = kb + q * 8;
+    const bool in = k < p.K;
+    const uint4 a = lo && in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : zero, c = hi && in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int m = n * 8 + g;
+      const uint4 b = in && m < p.M ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(m) * p.K + k)) : zero;
+      const uint32_t a0[4] = {a.x, c.x, a.y, c.y}, a1[4] = {a.z, c.z, a.w, c.w};
+      mma_bf16_16816(d[n], a0, b.x, b.y);
+      mma_bf16_16816(d[n], a1, b.z, b.w);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {  // rows g, g + 8 of the outputs, columns 2 q, 2 q + 1 of x's rows
+    s_sum[warp][n * 8 + 2 * q][g] = d[n][0];
+    s_sum[warp][n * 8 + 2 * q + 1][g] = d[n][1];
+    s_sum[warp][n * 8 + 2 * q][g + 8] = d[n][2];
+    s_sum[warp][n * 8 + 2 * q + 1][g + 8] = d[n][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NB * 8 * 8; i += kRowsWarps * 32) {  // two neighbouring outputs of a row
+    const int m = i >> 3, jl = (i & 7) * 2, j = j0 + jl;
+    if (m >= p.M || j >= p.N) continue;
+    float v[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kRowsWarps; ++u) { v[0] += s_sum[u][m][jl]; v[1] += s_sum[u][m][jl + 1]; }
+    if (p.bias != nullptr) {
+      if (p.bias_bf16) {
+        const uint32_t b = __ldg(reinterpret_cast<const unsigned*>(static_cast<const __nv_bfloat16*>(p.bias) + j));
+        v[0] += bf16_lo(b); v[1] += bf16_hi(b);
+      } else {
+        v[0] += __ldg(static_cast<const float*>(p.bias) + j); v[1] += __ldg(static_cast<const float*>(p.bias) + j + 1);
+      }
+    }
+    const size_t at = static_cast<size_t>(m) * p.N + j;
+    if (z != nullptr)
+      *reinterpret_cast<uint32_t*>(z + at) = ACT == FRNN_ACT_RELU ? (v[0] > 0.0f ? 0x3c00u : 0u) | (v[1] > 0.0f ? 0x3c000000u : 0u) : pack_half2(v[0], v[1]);
+    act_pair<ACT>(v[0], v[1]);
+    if (residual != nullptr) {
+      const uint32_t r = __ldg(reinterpret_cast<const unsigned*>(residual + at));
+      v[0] += bf16_lo(r); v[1] += bf16_hi(r);
+    }
+    *reinterpret_cast<uint32_t*>(out + at) = pack_bf16x2(v[0], v[1]);
+  }
+}
+
 // dz = dy act'(z) (not stored where the activation is none: dz = dy), and the columns' sums of a block's rows for dbias.
 constexpr int kSlopeRows = 64;
 template <int ACT>
 __global__ void __launch_bounds__(256) product_slope_kernel(const __nv_bfloat16* __restrict__ dy, const __half* __restrict__ z,
                                                             __nv_bfloat16* __restrict__ dz, float* __restrict__ part, int M, int N) {
+  constexpr int kBatch = 4;  // rows of a warp whose loads are in flight together
   __shared__ float s_sum[8][32][9];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.y * 32 + lane) * 8;
-  const int m_end = min((static_cast<int>(blockIdx.x) + 1) * kSlopeRows, M);
+  const long long m0 = static_cast<long long>(blockIdx.x) * kSlopeRows + warp;
   float sum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
   if (j < N) {
-#pragma unroll 4
-    for (int m = blockIdx.x * kSlopeRows + warp; m < m_end; m += 8) {
-      const long long at = static_cast<long long>(m) * N + j;
-      const uint4 g = __ldg(reinterpret_cast<const uint4*>(dy + at));
-      float v[8] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y), bf16_lo(g.z), bf16_hi(g.z), bf16_lo(g.w), bf16_hi(g.w)};
-      if constexpr (ACT != FRNN_ACT_NONE) {
-        const uint4 h = __ldg(reinterpret_cast<const uint4*>(z + at));
-        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-          v[2 * e] *= act_slope<ACT>(f.x);
-          v[2 * e + 1] *= act_slope<ACT>(f.y);
+    for (int r = 0; r < kSlopeRows / 8; r += kBatch) {
+      uint4 g[kBatch], h[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const long long m = m0 + (r + i) * 8;
+        g[i] = h[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (m < M) {
+          g[i] = __ldg(reinterpret_cast<const uint4*>(dy + m * N + j));
+          if constexpr (ACT != FRNN_ACT_NONE) h[i] = __ldg(reinterpret_cast<const uint4*>(z + m * N + j));
         }
-        *reinterpret_cast<uint4*>(dz + at) =
-            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += v[e];
+      for (int i = 0; i < kBatch; ++i) {
+        const long long m = m0 + (r + i) * 8;
+        if (m >= M) break;
+        float v[8] = {bf16_lo(g[i].x), bf16_hi(g[i].x), bf16_lo(g[i].y), bf16_hi(g[i].y), bf16_lo(g[i].z), bf16_hi(g[i].z), bf16_lo(g[i].w), bf16_hi(g[i].w)};
+        if constexpr (ACT != FRNN_ACT_NONE) {
+          const uint32_t w[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            v[2 * e] *= act_slope<ACT>(f.x);
+            v[2 * e + 1] *= act_slope<ACT>(f.y);
+          }
+          *reinterpret_cast<uint4*>(dz + m * N + j) =
+              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+      }
     }
   }
   if (part == nullptr) return;
@@ -564,32 +664,34 @@ __global__ void __launch_bounds__(1024) product_bias_kernel(const float* __restr
   }
 }
 
-// How an M x N x K product is cut: columns of a tile, parts of K.
-struct Cut { int np, parts, chunks_per_part; };
+// How an M x N x K product is cut: columns of a tile; tiles done whole, the rest in parts of K.
+struct Cut { int np, parts, chunks_per_part; long long whole, rest; };
 Cut choose_cut(long long M, long long N, long long K) {
   const long long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, mt = (M + 255) / 256, chunks = (K + kKC - 1) / kKC;
   Cut best{};
-  double best_t = 0;
+  double best_us = 0;
   for (int np = 256; np >= 128; np -= 64) {
-    const long long tiles = mt * ((N + np - 1) / np);
+    // Measured: 64 k's of a tile of 256, 192, 128 columns take 0.40, 0.39, 0.36 us (what a stage takes to arrive, not the tensor
+    // cores, sets the narrow ones'), the pass over the parts' sums 2.5 us and their bytes, written and read, at 4 TB/s.
+    const double chunk_us = np == 256 ? 0.40 : (np == 192 ? 0.39 : 0.36);
+    const long long tiles = mt * ((N + np - 1) / np), whole = tiles / pairs * pairs, rest = tiles - whole;
     for (long long parts = 1; parts <= 16 && parts <= chunks; ++parts) {
       const long long cpp = (chunks + parts - 1) / parts;
       if ((chunks + cpp - 1) / cpp != parts) continue;
-      const long long waves = (tiles * parts + pairs - 1) / pairs;
-      // cycles: 64 k's of a tile, filling and draining, the pass over partial sums (4 bytes written and read)
-      double t = static_cast<double>(waves) * cpp * (np == 256 ? 600 : np == 192 ? 480 : 400) + 3000;
-      if (parts > 1) t += 5000 + static_cast<double>(M) * N * parts * 8 / 2500;
-      if (best.np == 0 || t < best_t) {
-        best = {np, static_cast<int>(parts), static_cast<int>(cpp)};
-        best_t = t;
+      double us = static_cast<double>(whole / pairs) * chunks * chunk_us + static_cast<double>((rest * parts + pairs - 1) / pairs) * cpp * chunk_us;
+      if (parts > 1) us += 2.5 + static_cast<double>(rest) * parts * 256 * np * 8 / 4e6;
+      if (best.np == 0 || us < best_us) {
+        best = parts > 1 ? Cut{np, static_cast<int>(parts), static_cast<int>(cpp), whole, rest} : Cut{np, 1, static_cast<int>(chunks), tiles, 0};
+        best_us = us;
       }
+      if (rest == 0) break;
     }
   }
   return best;
 }
 long long work_bytes(long long M, long long N, long long K) {
   const Cut c = choose_cut(M, N, K);
-  return c.parts > 1 ? 4 * M * N * c.parts : 0;
+  return 4 * c.rest * c.parts * 256 * c.np;
 }
 
 int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long long rows, uint32_t box_cols, uint32_t box_rows) {
@@ -598,25 +700,25 @@ int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long lo
   return make_tensor_map(map, base, elem, 2, dims, box, true);
 }
 
-template <bool A_MN, bool B_MN, int NP, bool PARTIAL, int ACT>
-int launch_kernel(const ProductParams& p, const CUtensorMap (&maps)[5], cudaStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, PARTIAL, ACT>);
+template <bool A_MN, bool B_MN, int NP, int ACT>
+int launch_kernel(const ProductParams& p, const CUtensorMap (&maps)[6], cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, ACT>);
   cudaError_t e = raise_limits(kern, smem_of(NP, B_MN), false);
   if (e != cudaSuccess) return static_cast<int>(e);
   const long long pairs = sm_count() / 2;
-  const unsigned grid = 2u * static_cast<unsigned>(p.n_tiles < pairs ? p.n_tiles : pairs);
-  product_kernel<A_MN, B_MN, NP, PARTIAL, ACT><<<grid, kThreads, smem_of(NP, B_MN), s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
+  const unsigned grid = 2u * static_cast<unsigned>(p.n_units < pairs ? p.n_units : pairs);
+  product_kernel<A_MN, B_MN, NP, ACT><<<grid, kThreads, smem_of(NP, B_MN), s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5]);
   return static_cast<int>(cudaGetLastError());
 }
 // The gradients' products have no epilogue.
 template <bool A_MN, bool B_MN, int NP>
-int launch_act(const ProductParams& p, const CUtensorMap (&maps)[5], cudaStream_t s) {
+int launch_act(const ProductParams& p, const CUtensorMap (&maps)[6], cudaStream_t s) {
   if constexpr (!A_MN && !B_MN) {
-    if (p.act == FRNN_ACT_RELU) return launch_kernel<false, false, NP, false, FRNN_ACT_RELU>(p, maps, s);
-    if (p.act == FRNN_ACT_SILU) return launch_kernel<false, false, NP, false, FRNN_ACT_SILU>(p, maps, s);
-    if (p.act == FRNN_ACT_GELU_TANH) return launch_kernel<false, false, NP, false, FRNN_ACT_GELU_TANH>(p, maps, s);
+    if (p.act == FRNN_ACT_RELU) return launch_kernel<false, false, NP, FRNN_ACT_RELU>(p, maps, s);
+    if (p.act == FRNN_ACT_SILU) return launch_kernel<false, false, NP, FRNN_ACT_SILU>(p, maps, s);
+    if (p.act == FRNN_ACT_GELU_TANH) return launch_kernel<false, false, NP, FRNN_ACT_GELU_TANH>(p, maps, s);
   }
-  return launch_kernel<A_MN, B_MN, NP, false, FRNN_ACT_NONE>(p, maps, s);
+  return launch_kernel<A_MN, B_MN, NP, FRNN_ACT_NONE>(p, maps, s);
 }
 
 // C [M][N] = A . B with the epilogue of `p` (bias, act); A [M][K] or, A_MN, [K][M]; B [N][K] or, B_MN, [K][N].
@@ -625,45 +727,55 @@ int product_launch(ProductParams p, const void* A, const void* B, long long M, l
                    void* z, float* work, cudaStream_t s) {
   const Cut cut = choose_cut(M, N, K);
   p.M = static_cast<int>(M); p.N = static_cast<int>(N); p.K = static_cast<int>(K);
-  p.n_mt = static_cast<int>((M + 255) / 256); p.n_nt = static_cast<int>((N + cut.np - 1) / cut.np);
-  p.chunks = static_cast<int>((K + kKC - 1) / kKC); p.chunks_per_split = cut.chunks_per_part;
-  p.n_tiles = static_cast<long long>(p.n_mt) * p.n_nt * cut.parts;
+  p.n_nt = static_cast<int>((N + cut.np - 1) / cut.np);
+  p.chunks = static_cast<int>((K + kKC - 1) / kKC);
+  p.parts = cut.parts; p.chunks_per_part = cut.chunks_per_part;
+  p.whole = cut.whole; p.n_units = cut.whole + cut.rest * cut.parts;
   p.has_residual = residual != nullptr; p.has_z = z != nullptr;
-  CUtensorMap maps[5];
+  if (cut.rest > 0 && work == nullptr) return -5;
+  CUtensorMap maps[6];
   const uint32_t half = static_cast<uint32_t>(cut.np / 2);
   int rc = A_MN ? map_2d(&maps[0], A, 2, M, K, 64, kKC) : map_2d(&maps[0], A, 2, K, M, kKC, 128);
   if (rc == 0) rc = B_MN ? map_2d(&maps[1], B, 2, N, K, 64, kKC) : map_2d(&maps[1], B, 2, K, N, kKC, half);
-  if (rc != 0) return rc;
-  if (cut.parts > 1) {
-    if (work == nullptr) return -5;
-    const uint64_t dims[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(cut.parts)};
-    const uint32_t box[3] = {32, 32, 1};
-    rc = make_tensor_map(&maps[2], work, 4, 3, dims, box, true);
-    if (rc != 0) return rc;
-    maps[3] = maps[4] = maps[2];
-    rc = cut.np == 256   ? launch_kernel<A_MN, B_MN, 256, true, FRNN_ACT_NONE>(p, maps, s)
-         : cut.np == 192 ? launch_kernel<A_MN, B_MN, 192, true, FRNN_ACT_NONE>(p, maps, s)
-                         : launch_kernel<A_MN, B_MN, 128, true, FRNN_ACT_NONE>(p, maps, s);
-    if (rc != 0) return rc;
-    const unsigned blocks = static_cast<unsigned>((M * N / 8 + 255) / 256);
-    const auto* r = static_cast<const __nv_bfloat16*>(residual);
-    auto* o = static_cast<__nv_bfloat16*>(out);
-    auto* keep = static_cast<uint4*>(z);
-    if (p.act == FRNN_ACT_RELU) product_join_kernel<FRNN_ACT_RELU><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
-    else if (p.act == FRNN_ACT_SILU) product_join_kernel<FRNN_ACT_SILU><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
-    else if (p.act == FRNN_ACT_GELU_TANH) product_join_kernel<FRNN_ACT_GELU_TANH><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
-    else product_join_kernel<FRNN_ACT_NONE><<<blocks, 256, 0, s>>>(p, work, cut.parts, r, o, keep);
-    return static_cast<int>(cudaGetLastError());
-  }
-  rc = map_2d(&maps[2], out, 2, N, M, 64, 32);
+  if (rc == 0) rc = map_2d(&maps[2], out, 2, N, M, 64, 32);
   if (rc == 0 && residual != nullptr) rc = map_2d(&maps[3], residual, 2, N, M, 64, 32);
   if (rc == 0 && z != nullptr) rc = map_2d(&maps[4], z, 2, N, M, 64, 32);
+  if (rc == 0 && cut.rest > 0) rc = map_2d(&maps[5], work, 4, cut.np, cut.rest * cut.parts * 256, 32, 32);
   if (rc != 0) return rc;
   if (residual == nullptr) maps[3] = maps[2];
   if (z == nullptr) maps[4] = maps[2];
-  return cut.np == 256   ? launch_act<A_MN, B_MN, 256>(p, maps, s)
-         : cut.np == 192 ? launch_act<A_MN, B_MN, 192>(p, maps, s)
-                         : launch_act<A_MN, B_MN, 128>(p, maps, s);
+  if (cut.rest == 0) maps[5] = maps[2];
+  rc = cut.np == 256   ? launch_act<A_MN, B_MN, 256>(p, maps, s)
+       : cut.np == 192 ? launch_act<A_MN, B_MN, 192>(p, maps, s)
+                       : launch_act<A_MN, B_MN, 128>(p, maps, s);
+  if (rc != 0 || cut.rest == 0) return rc;
+  const unsigned blocks = static_cast<unsigned>(cut.rest * (cut.np / 8));
+  const auto* r = static_cast<const __nv_bfloat16*>(residual);
+  auto* o = static_cast<__nv_bfloat16*>(out);
+  auto* keep = static_cast<uint4*>(z);
+  if (p.act == FRNN_ACT_RELU) product_join_kernel<FRNN_ACT_RELU><<<blocks, 256, 0, s>>>(p, work, cut.np, r, o, keep);
+  else if (p.act == FRNN_ACT_SILU) product_join_kernel<FRNN_ACT_SILU><<<blocks, 256, 0, s>>>(p, work, cut.np, r, o, keep);
+  else if (p.act == FRNN_ACT_GELU_TANH) product_join_kernel<FRNN_ACT_GELU_TANH><<<blocks, 256, 0, s>>>(p, work, cut.np, r, o, keep);
+  else product_join_kernel<FRNN_ACT_NONE><<<blocks, 256, 0, s>>>(p, work, cut.np, r, o, keep);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <int ACT>
+int rows_act(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((p.N + 15) / 16);
+  const auto *a = static_cast<const __nv_bfloat16*>(x), *b = static_cast<const __nv_bfloat16*>(w), *r = static_cast<const __nv_bfloat16*>(residual);
+  auto* o = static_cast<__nv_bfloat16*>(y);
+  auto* h = static_cast<__half*>(z);
+  if (p.M <= 8) product_rows_kernel<ACT, 1><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
+  else if (p.M <= 16) product_rows_kernel<ACT, 2><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
+  else product_rows_kernel<ACT, 4><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
+  return static_cast<int>(cudaGetLastError());
+}
+int rows_launch(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
+  if (p.act == FRNN_ACT_RELU) return rows_act<FRNN_ACT_RELU>(p, x, w, residual, y, z, s);
+  if (p.act == FRNN_ACT_SILU) return rows_act<FRNN_ACT_SILU>(p, x, w, residual, y, z, s);
+  if (p.act == FRNN_ACT_GELU_TANH) return rows_act<FRNN_ACT_GELU_TANH>(p, x, w, residual, y, z, s);
+  return rows_act<FRNN_ACT_NONE>(p, x, w, residual, y, z, s);
 }
 
 bool bad_sizes(int64_t rows, int outputs, int inputs) { return rows < 1 || outputs < 1 || inputs < 1; }
@@ -684,7 +796,8 @@ extern "C" int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frn
   if (out == nullptr || bad_sizes(rows, outputs, inputs)) return -5;
   if (unsupported(rows, outputs, inputs)) return -2;
   *out = {};
-  out->forward_work_bytes = work_bytes(rows, outputs, inputs);
+  out->forward_waits = rows > kRowsMax;
+  if (out->forward_waits) out->forward_work_bytes = work_bytes(rows, outputs, inputs);
   const long long dx = work_bytes(rows, inputs, outputs), dw = work_bytes(outputs, inputs, rows);
   out->backward_work_bytes = dx > dw ? dx : dw;
   out->dbpart_bytes = 4 * ((rows + kSlopeRows - 1) / kSlopeRows) * outputs;
@@ -694,11 +807,15 @@ extern "C" int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frn
 extern "C" int frnn_b200_product_forward(const void* x, const void* w, const void* bias, int bias_bf16, const void* residual, int activation,
                                          void* y, void* z, int64_t rows, int outputs, int inputs, float* work, int* err, void* stream) {
   using namespace frnn;
-  if (!x || !w || !y || !err || bad_sizes(rows, outputs, inputs) || bad_act(activation)) return -5;
+  if (!x || !w || !y || bad_sizes(rows, outputs, inputs) || bad_act(activation) || (!err && rows > kRowsMax)) return -5;
   if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias) || misaligned(residual) || misaligned(z) || misaligned(work)) return -5;
   if (unsupported(rows, outputs, inputs)) return -2;
   ProductParams p{};
   p.bias = bias; p.bias_bf16 = bias_bf16; p.act = activation; p.err = err;
+  if (rows <= kRowsMax) {
+    p.M = static_cast<int>(rows); p.N = outputs; p.K = inputs;
+    return rows_launch(p, x, w, residual, y, z, static_cast<cudaStream_t>(stream));
+  }
   return product_launch<false, false>(p, x, w, rows, outputs, inputs, residual, y, z, work, static_cast<cudaStream_t>(stream));
 }
 

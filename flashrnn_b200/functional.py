@@ -70,6 +70,7 @@ class _ErrorBlock:
     def __init__(self, device, stream):
         self.stream, self.event = stream, torch.cuda.Event()
         self.words = torch.zeros((self.SIZE, 32), dtype=torch.int32, device=device)
+        self.address = self.words.data_ptr()
         self.names = []      # of the words tracked, in order
         self.closed = 0      # words that are in the queue
         self.given = 0
@@ -88,6 +89,14 @@ def _error_word(device: torch.device) -> torch.Tensor:
     """32 zeroed words for a launch of this thread on the device's current stream; goes to ``_track`` after the launch."""
     if _capturing():
         return torch.zeros(32, dtype=torch.int32, device=device)   # zeroed by every replay
+    block, i = _take_word(device)
+    word = block.words[i]
+    word._frnn_block = block
+    return word
+
+
+def _take_word(device: torch.device):
+    """(block, index) of the next word of this thread on the device's current stream"""
     key = (threading.get_ident(), device.index, _stream(device))
     with _blocks_lock:
         block = _blocks.get(key)
@@ -97,10 +106,27 @@ def _error_word(device: torch.device) -> torch.Tensor:
             block = _blocks[key] = _ErrorBlock(device, torch.cuda.current_stream(device))
         if len(block.names) < block.given:        # a launch that was refused after it had taken its word: it is free again
             block.given = len(block.names)
-        word = block.words[block.given]
         block.given += 1
-    word._frnn_block = block
-    return word
+        return block, block.given - 1
+
+
+def _launch_word(device: torch.device):
+    """What ``_error_word`` gives, as (address, what to hand to ``_launched``): a tensor for the word costs as much as its event."""
+    if _capturing():
+        word = torch.zeros(32, dtype=torch.int32, device=device)
+        return word.data_ptr(), word
+    block, i = _take_word(device)
+    return block.address + 128 * i, block
+
+
+def _launched(holder, what: str) -> None:
+    """``_track`` for ``_launch_word``"""
+    if not isinstance(holder, _ErrorBlock):
+        _track(holder, what)
+        return
+    with _blocks_lock:
+        holder.event.record(holder.stream)
+        holder.names.append(what)
 
 
 _captured_errors: list = []   # error words of launches recorded into CUDA graphs: (err, what), newest last

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import _dense, _error_word, _ptr, _stream, _track, poll_errors
+from .functional import _dense, _launch_word, _launched, _ptr, _stream, poll_errors
 
 # function -> gates of Wx and b
 LINEAR_GATES = {"leaky": 2, "lstm": 4}
@@ -31,21 +31,22 @@ def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Option
     B, T, _, N, D = wx.shape
     dev = wx.device
     plan = _lib.linear_plan(function, B, T, N, D)
-    hidden = torch.empty((B, T, N, D), dtype=wx.dtype, device=dev)
+    hidden = wx.new_empty((B, T, N, D))
     if last is None:
-        last = torch.empty((1, B, 1, N, D), dtype=torch.float32, device=dev)
-    starts = exchange = err = None
+        last = bias.new_empty((1, B, 1, N, D))
+    starts = exchange = err = word = None
     if keep and plan.starts_bytes:
-        starts = torch.empty(plan.starts_bytes // 4, dtype=torch.float32, device=dev)
+        starts = bias.new_empty(plan.starts_bytes // 4)
     if plan.exchange_bytes:   # several tiles, which wait for one another
-        exchange, err = torch.empty(plan.exchange_bytes, dtype=torch.uint8, device=dev), _error_word(dev)
+        exchange = bias.new_empty(plan.exchange_bytes // 4)
+        err, word = _launch_word(dev)
     rc = lib.frnn_b200_linear_forward(
         _lib.LINEAR_CELLS[function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
-        hidden.data_ptr(), last.data_ptr(), _ptr(starts), _ptr(exchange), B, T, N, D, 0, _ptr(err), _stream(dev))
+        hidden.data_ptr(), last.data_ptr(), _ptr(starts), _ptr(exchange), B, T, N, D, 0, err, _stream(dev))
     if rc:
         _lib.check(rc, "frnn_b200_linear_forward")
     if err is not None:
-        _track(err, "frnn_b200_linear_forward")
+        _launched(word, "frnn_b200_linear_forward")
     return hidden, last, starts
 
 
@@ -76,25 +77,26 @@ class _LinearRecurrence(torch.autograd.Function):
         poll_errors()
         B, T, _, N, D = wx.shape
         plan = _lib.linear_plan(ctx.function, B, T, N, D)
-        d_hidden = torch.zeros((B, T, N, D), dtype=wx.dtype, device=dev) if d_hidden is None else _dense(d_hidden)
+        d_hidden = wx.new_zeros((B, T, N, D)) if d_hidden is None else _dense(d_hidden)
         if d_last is not None:
             d_last = d_last.contiguous()
         d_wx, db = torch.empty_like(wx), torch.empty_like(bias)
         need = ctx.needs_input_grad
         d_initial = torch.empty_like(initial) if need[2] else None
-        part = exchange = err = None
+        part = exchange = err = word = None
         if plan.dbpart_bytes:   # and the exchange buffer, whose size is 0 where there is nothing to wait for, in one allocation
-            room = (plan.exchange_bytes + 15) // 16 * 16
-            scratch = torch.empty(room + plan.dbpart_bytes, dtype=torch.uint8, device=dev)
+            room = plan.exchange_bytes
+            scratch = bias.new_empty((room + plan.dbpart_bytes) // 4)
             part = scratch.data_ptr() + room
             if room:
-                exchange, err = scratch.data_ptr(), _error_word(dev)
+                exchange = scratch.data_ptr()
+                err, word = _launch_word(dev)
         rc = lib.frnn_b200_linear_backward(
             _lib.LINEAR_CELLS[ctx.function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
             _ptr(starts), d_hidden.data_ptr(), _ptr(d_last), d_wx.data_ptr(), db.data_ptr(), _ptr(d_initial), part, exchange,
-            B, T, N, D, 0, _ptr(err), _stream(dev))
+            B, T, N, D, 0, err, _stream(dev))
         if err is not None:
-            _track(err, "frnn_b200_linear_backward")   # the scan has the word, whether the sum of db behind it was accepted or not
+            _launched(word, "frnn_b200_linear_backward")   # the scan has the word, whether the sum of db behind it was accepted or not
         if rc:
             _lib.check(rc, "frnn_b200_linear_backward")
         return d_wx if need[0] else None, db if need[1] else None, d_initial, None, None

@@ -21,7 +21,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import SIZES, FlashRNNConfig, _dense, _error_word, _ptr, _stream, _track, flashrnn, poll_errors
+from .functional import SIZES, FlashRNNConfig, _dense, _error_word, _launch_word, _launched, _ptr, _stream, _track, flashrnn, poll_errors
 from .linear import _current_device, _refuse_second_derivative
 
 
@@ -104,16 +104,17 @@ def _product_forward(x, weight, bias, residual, activation, keep: bool):
     poll_errors()
     (M, I), J, dev = x.shape, weight.shape[0], x.device
     plan = _lib.product_plan(M, J, I, dev.index)
-    y = torch.empty((M, J), dtype=torch.bfloat16, device=dev)
+    y = x.new_empty((M, J))
     z = torch.empty((M, J), dtype=torch.float16, device=dev) if keep and activation is not None else None
     work = torch.empty(plan.forward_work_bytes // 4, dtype=torch.float32, device=dev) if plan.forward_work_bytes else None
-    err = _error_word(dev)
+    err, word = _launch_word(dev) if plan.forward_waits else (None, None)
     rc = lib.frnn_b200_product_forward(
         x.data_ptr(), weight.data_ptr(), _ptr(bias), bias is not None and bias.dtype == torch.bfloat16, _ptr(residual),
-        _lib.ACTIVATIONS[activation], y.data_ptr(), _ptr(z), M, J, I, _ptr(work), err.data_ptr(), _stream(dev))
+        _lib.ACTIVATIONS[activation], y.data_ptr(), _ptr(z), M, J, I, _ptr(work), err, _stream(dev))
     if rc:
         _lib.check(rc, "frnn_b200_product_forward")
-    _track(err, "frnn_b200_product_forward")
+    if word is not None:
+        _launched(word, "frnn_b200_product_forward")
     return y, z
 
 
@@ -146,8 +147,8 @@ class _FusedProjection(torch.autograd.Function):
         M, I, J = ctx.sizes
         plan = _lib.product_plan(M, J, I, dev.index)
         g = _dense(dy)
-        dx = torch.empty((M, I), dtype=torch.bfloat16, device=dev) if need_x else None
-        dw = torch.empty((J, I), dtype=torch.bfloat16, device=dev) if need_w else None
+        dx = g.new_empty((M, I)) if need_x else None
+        dw = g.new_empty((J, I)) if need_w else None
         db = torch.empty(J, dtype=ctx.bias_dtype, device=dev) if need_b else None
         # dz, the partial sums of dbias and of the products: one allocation, each part on a 16-byte boundary
         dz_bytes = 2 * M * J if z is not None else 0
@@ -157,12 +158,12 @@ class _FusedProjection(torch.autograd.Function):
         if total:
             scratch = torch.empty(total, dtype=torch.uint8, device=dev)
             at = scratch.data_ptr()
-        err = _error_word(dev)
+        err, word = _launch_word(dev)
         rc = lib.frnn_b200_product_backward(
             g.data_ptr(), _ptr(z), _ptr(x), _ptr(weight), _lib.ACTIVATIONS[ctx.activation], at if dz_bytes else None, _ptr(dx), _ptr(dw),
             _ptr(db), ctx.bias_dtype == torch.bfloat16, at + dz_bytes if part_bytes else None, M, J, I,
-            at + dz_bytes + part_bytes if plan.backward_work_bytes else None, err.data_ptr(), _stream(dev))
-        _track(err, "frnn_b200_product_backward")   # earlier launches of the call have the word, whether a later one was accepted or not
+            at + dz_bytes + part_bytes if plan.backward_work_bytes else None, err, _stream(dev))
+        _launched(word, "frnn_b200_product_backward")   # earlier launches of the call have the word, whether a later one was accepted or not
         if rc:
             _lib.check(rc, "frnn_b200_product_backward")
         return dx, dw, db, dy if need_r else None, None

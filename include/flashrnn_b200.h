@@ -254,6 +254,7 @@ enum { FRNN_ACT_NONE = 0, FRNN_ACT_RELU = 1, FRNN_ACT_SILU = 2, FRNN_ACT_GELU_TA
 typedef struct frnn_b200_product_plan {
   int64_t forward_work_bytes, backward_work_bytes;  /* fp32 partial sums of products with few tiles (0: work may be NULL) */
   int64_t dbpart_bytes;                             /* scratch for dbias                                                  */
+  int forward_waits;                                /* 0: nothing in the forward call waits, err may be NULL              */
 } frnn_b200_product_plan_t;
 
 /* On the current device (how a product is cut depends on its SM count). */

@@ -47,7 +47,7 @@ def test_c_entries_refuse_before_any_launch():
     lib = _lib.load()
     f = lambda x=16, w=16, bias=16, y=16, act=1, M=8, J=8, I=8, err=16: lib.frnn_b200_product_forward(  # noqa: E731
         x, w, bias, 1, None, act, y, None, M, J, I, None, err, None)
-    assert f(x=None) == f(w=None) == f(y=None) == f(err=None) == f(act=4) == f(M=0) == f(x=8) == f(bias=4) == f(y=24) == -5
+    assert f(x=None) == f(w=None) == f(y=None) == f(err=None, M=33) == f(act=4) == f(M=0) == f(x=8) == f(bias=4) == f(y=24) == -5
     assert f(J=12) == f(I=4) == f(M=1 << 31) == -2
     g = lambda dy=16, z=16, x=16, w=16, act=1, dz=16, dx=16, part=16, I=8: lib.frnn_b200_product_backward(  # noqa: E731
         dy, z, x, w, act, dz, dx, 16, 16, 1, part, 8, 8, I, None, 16, None)

@@ -38,7 +38,8 @@ def step(function, wx, b, s, n, dh, dl):
 
 # one step; less than, exactly and just over a span of four or eight, a tile of 128; channels that end inside a block of 64 or
 # 32; widths that are no multiple of four; two tiles and more; more than one group of 16 tiles
-SHAPES = [(1, 1, 1, 1), (4, 1, 3, 256), (2, 3, 1, 7), (3, 4, 1, 64), (2, 5, 2, 34), (2, 9, 1, 33), (1, 64, 1, 72), (2, 127, 1, 20),
+SHAPES = [(1, 1, 1, 1), (4, 1, 3, 256), (2, 3, 1, 7), (3, 4, 1, 64), (2, 5, 2, 34), (2, 9, 1, 33), (3, 17, 1, 68), (2, 18, 1, 31),
+          (2, 33, 1, 130), (1, 64, 1, 72), (2, 127, 1, 20),
           (2, 128, 1, 65), (2, 129, 2, 32), (3, 300, 1, 36), (1, 385, 1, 5), (1, 2048, 1, 4), (1, 2049, 1, 3), (2, 4500, 1, 8)]
 
 
