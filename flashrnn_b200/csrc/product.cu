@@ -15,7 +15,7 @@
 // the MMAs of both, 8 warps of each CTA take the accumulator out of tensor memory: two accumulators, so the epilogue of a tile
 // runs under the contraction of the next. Rows and columns past the edges are read as zeros and not stored.
 // Tiles that do not fill another round of all pairs are cut along K, so that their parts do: these go out in fp32 and are summed in
-// order by product_join_kernel, which then has the epilogue. Up to 32 rows take product_rows_kernel, which reads W once from registers.
+// order by product_join_kernel, which then has the epilogue. Few rows take product_rows_kernel.
 #include "../../include/flashrnn_b200.h"
 
 #include "frnn_common.cuh"
@@ -518,18 +518,17 @@ __global__ void __launch_bounds__(256) product_join_kernel(const ProductParams p
   *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// Up to 32 rows: W is read once, from where it lies into the registers of mma.sync (16 outputs x 16 k's), the rows of x are the other
-// operand, eight to an instruction. The tensor pipe's rate does not matter here, the time to get W does: a warp has an eighth of K and
-// all of its loads in flight. The order of k's inside a product is free as long as both operands have the same: a lane takes 16 bytes, eight
+// Few rows: W goes from where it lies into the registers of mma.sync (16 outputs x 16 k's), the rows of x are the other operand,
+// eight to an instruction, 32 to a CTA. The tensor pipe's rate does not matter here, the time to get W does: a warp has an eighth (a
+// sixteenth) of K and its loads in flight together. 1 x 4096 x 4096 takes 10.3 us (3.3 TB/s; a library product 12.9). The order of k's inside a product is free as long as both operands have the same: a lane takes 16 bytes, eight
 // neighbouring k's, which are two instructions' fragments.
-constexpr int kRowsMax = 32, kRowsWarps = 8;
-template <int ACT, int NB>
-__global__ void __launch_bounds__(kRowsWarps * 32) product_rows_kernel(const ProductParams p, const __nv_bfloat16* __restrict__ x,
+template <int ACT, int NB, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) product_rows_kernel(const ProductParams p, const __nv_bfloat16* __restrict__ x,
                                                                      const __nv_bfloat16* __restrict__ w,
                                                                      const __nv_bfloat16* __restrict__ residual,
                                                                      __nv_bfloat16* __restrict__ out, __half* __restrict__ z) {
-  __shared__ float s_sum[kRowsWarps][NB * 8][17];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, j0 = blockIdx.x * 16;
+  __shared__ float s_sum[WARPS][NB * 8][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, j0 = blockIdx.x * 16, m0 = blockIdx.y * NB * 8;
   float d[NB][4];
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -539,13 +538,13 @@ __global__ void __launch_bounds__(kRowsWarps * 32) product_rows_kernel(const Pro
   const bool lo = j0 + g < p.N, hi = j0 + g + 8 < p.N;
   const __nv_bfloat16 *w0 = w + static_cast<size_t>(j0 + g) * p.K, *w1 = w0 + static_cast<size_t>(8) * p.K;
 #pragma unroll 4
-  for (int kb = warp * 32; kb < p.K; kb += kRowsWarps * 32) {
+  for (int kb = warp * 32; kb < p.K; kb += WARPS * 32) {
     const int k = kb + q * 8;
     const bool in = k < p.K;
     const uint4 a = lo && in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : zero, c = hi && in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : zero;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int m = n * 8 + g;
+      const int m = m0 + n * 8 + g;
       const uint4 b = in && m < p.M ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(m) * p.K + k)) : zero;
       const uint32_t a0[4] = {a.x, c.x, a.y, c.y}, a1[4] = {a.z, c.z, a.w, c.w};
       mma_bf16_16816(d[n], a0, b.x, b.y);
@@ -560,12 +559,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32) product_rows_kernel(const Pro
     s_sum[warp][n * 8 + 2 * q + 1][g + 8] = d[n][3];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < NB * 8 * 8; i += kRowsWarps * 32) {  // two neighbouring outputs of a row
-    const int m = i >> 3, jl = (i & 7) * 2, j = j0 + jl;
+  for (int i = threadIdx.x; i < NB * 8 * 8; i += WARPS * 32) {  // two neighbouring outputs of a row
+    const int ml = i >> 3, m = m0 + ml, jl = (i & 7) * 2, j = j0 + jl;
     if (m >= p.M || j >= p.N) continue;
     float v[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int u = 0; u < kRowsWarps; ++u) { v[0] += s_sum[u][m][jl]; v[1] += s_sum[u][m][jl + 1]; }
+    for (int u = 0; u < WARPS; ++u) { v[0] += s_sum[u][ml][jl]; v[1] += s_sum[u][ml][jl + 1]; }
     if (p.bias != nullptr) {
       if (p.bias_bf16) {
         const uint32_t b = __ldg(reinterpret_cast<const unsigned*>(static_cast<const __nv_bfloat16*>(p.bias) + j));
@@ -760,16 +759,27 @@ int product_launch(ProductParams p, const void* A, const void* B, long long M, l
   return static_cast<int>(cudaGetLastError());
 }
 
-template <int ACT>
-int rows_act(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((p.N + 15) / 16);
+// Which products the kernel of few rows takes. Every 32 rows read W again, so its time grows with all three sizes, while a tile's start and
+// end alone are 6 us. us, against tiles and, in brackets, a library product without an epilogue: rows x inputs x outputs 8 x 768 x 1536
+// 2.5, 9.3 (3.5), 16 x 4096 x 4096 13.8, 17.5 (10.1), 32 x 1024 x 4096 6.1, 11.0 (3.6), 256 x 768 x 768 6.2, 9.9 (3.5); behind
+// the border 256 x 768 x 1536 10.7, 9.9, 32 x 4096 x 4096 23.6, 17.6.
+bool few_rows(long long M, long long N, long long K) { return M <= 16 || (M <= 256 && M * N <= (1 << 28) / K); }
+
+template <int ACT, int NB>
+int rows_warps(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.N + 15) / 16), static_cast<unsigned>((p.M + NB * 8 - 1) / (NB * 8)));
   const auto *a = static_cast<const __nv_bfloat16*>(x), *b = static_cast<const __nv_bfloat16*>(w), *r = static_cast<const __nv_bfloat16*>(residual);
   auto* o = static_cast<__nv_bfloat16*>(y);
   auto* h = static_cast<__half*>(z);
-  if (p.M <= 8) product_rows_kernel<ACT, 1><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
-  else if (p.M <= 16) product_rows_kernel<ACT, 2><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
-  else product_rows_kernel<ACT, 4><<<grid, kRowsWarps * 32, 0, s>>>(p, a, b, r, o, h);
+  if (p.K <= 1024) product_rows_kernel<ACT, NB, 8><<<grid, 256, 0, s>>>(p, a, b, r, o, h);
+  else product_rows_kernel<ACT, NB, 16><<<grid, 512, 0, s>>>(p, a, b, r, o, h);
   return static_cast<int>(cudaGetLastError());
+}
+template <int ACT>
+int rows_act(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
+  if (p.M <= 8) return rows_warps<ACT, 1>(p, x, w, residual, y, z, s);
+  if (p.M <= 16) return rows_warps<ACT, 2>(p, x, w, residual, y, z, s);
+  return rows_warps<ACT, 4>(p, x, w, residual, y, z, s);
 }
 int rows_launch(const ProductParams& p, const void* x, const void* w, const void* residual, void* y, void* z, cudaStream_t s) {
   if (p.act == FRNN_ACT_RELU) return rows_act<FRNN_ACT_RELU>(p, x, w, residual, y, z, s);
@@ -796,7 +806,7 @@ extern "C" int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frn
   if (out == nullptr || bad_sizes(rows, outputs, inputs)) return -5;
   if (unsupported(rows, outputs, inputs)) return -2;
   *out = {};
-  out->forward_waits = rows > kRowsMax;
+  out->forward_waits = !few_rows(rows, outputs, inputs);
   if (out->forward_waits) out->forward_work_bytes = work_bytes(rows, outputs, inputs);
   const long long dx = work_bytes(rows, inputs, outputs), dw = work_bytes(outputs, inputs, rows);
   out->backward_work_bytes = dx > dw ? dx : dw;
@@ -807,12 +817,13 @@ extern "C" int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frn
 extern "C" int frnn_b200_product_forward(const void* x, const void* w, const void* bias, int bias_bf16, const void* residual, int activation,
                                          void* y, void* z, int64_t rows, int outputs, int inputs, float* work, int* err, void* stream) {
   using namespace frnn;
-  if (!x || !w || !y || bad_sizes(rows, outputs, inputs) || bad_act(activation) || (!err && rows > kRowsMax)) return -5;
+  if (!x || !w || !y || bad_sizes(rows, outputs, inputs) || bad_act(activation) ) return -5;
   if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias) || misaligned(residual) || misaligned(z) || misaligned(work)) return -5;
   if (unsupported(rows, outputs, inputs)) return -2;
+  if (!err && !few_rows(rows, outputs, inputs)) return -5;
   ProductParams p{};
   p.bias = bias; p.bias_bf16 = bias_bf16; p.act = activation; p.err = err;
-  if (rows <= kRowsMax) {
+  if (few_rows(rows, outputs, inputs)) {
     p.M = static_cast<int>(rows); p.N = outputs; p.K = inputs;
     return rows_launch(p, x, w, residual, y, z, static_cast<cudaStream_t>(stream));
   }

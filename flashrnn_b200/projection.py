@@ -99,12 +99,13 @@ def flashrnn_projected(x, W, R, b, states=None, bias_w=None, function: str = "ls
 
 
 def _product_forward(x, weight, bias, residual, activation, keep: bool):
-    """x [M,I], weight [J,I], residual [M,J] -> y [M,J] and, where the backward pass needs it, what the slope is taken at."""
+    """x [..., I], weight [J,I], residual [..., J] -> y [..., J] and, where the backward pass needs it, what the slope is taken at."""
     lib = _lib.load()
     poll_errors()
-    (M, I), J, dev = x.shape, weight.shape[0], x.device
+    J, I = weight.shape
+    M, dev = x.numel() // I, x.device
     plan = _lib.product_plan(M, J, I, dev.index)
-    y = x.new_empty((M, J))
+    y = x.new_empty((*x.shape[:-1], J))
     z = torch.empty((M, J), dtype=torch.float16, device=dev) if keep and activation is not None else None
     work = torch.empty(plan.forward_work_bytes // 4, dtype=torch.float32, device=dev) if plan.forward_work_bytes else None
     err, word = _launch_word(dev) if plan.forward_waits else (None, None)
@@ -124,7 +125,7 @@ class _FusedProjection(torch.autograd.Function):
         need = ctx.needs_input_grad
         y, z = _product_forward(x, weight, bias, residual, activation, need[0] or need[1] or need[2])
         ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, z)
-        ctx.activation, ctx.sizes = activation, (*x.shape, weight.shape[0])
+        ctx.activation, ctx.shapes = activation, (x.shape, weight.shape)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
@@ -144,11 +145,13 @@ class _FusedProjection(torch.autograd.Function):
         lib = _lib.load()
         poll_errors()
         x, weight, z = ctx.saved_tensors
-        M, I, J = ctx.sizes
+        x_shape, w_shape = ctx.shapes
+        J, I = w_shape
+        M = dy.numel() // J
         plan = _lib.product_plan(M, J, I, dev.index)
         g = _dense(dy)
-        dx = g.new_empty((M, I)) if need_x else None
-        dw = g.new_empty((J, I)) if need_w else None
+        dx = g.new_empty(x_shape) if need_x else None
+        dw = g.new_empty(w_shape) if need_w else None
         db = torch.empty(J, dtype=ctx.bias_dtype, device=dev) if need_b else None
         # dz, the partial sums of dbias and of the products: one allocation, each part on a 16-byte boundary
         dz_bytes = 2 * M * J if z is not None else 0
@@ -220,11 +223,11 @@ def _bf16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _run_product(x, weight, bias, activation, residual, grad: bool):
-    shape, (J, I) = x.shape, weight.shape
-    x, weight = _bf16(x).reshape(-1, I), _bf16(weight)
+    J, I = weight.shape
+    x, weight = _bf16(x), _bf16(weight)
     if residual is not None:
-        residual = _bf16(residual).reshape(-1, J)
-    if bias is not None and bias.dtype != torch.bfloat16:
+        residual = _bf16(residual)
+    if bias is not None and bias.dtype != torch.bfloat16 and bias.dtype != torch.float32:
         bias = bias.to(torch.float32)
     pad_i, pad_j = -I % 8, -J % 8
     if pad_i or pad_j:
@@ -241,4 +244,4 @@ def _run_product(x, weight, bias, activation, residual, grad: bool):
         y = _FusedProjection.apply(x, weight, bias, residual, activation)
     else:
         y = _product_forward(x, weight, bias, residual, activation, False)[0]
-    return (y[:, :J] if pad_j else y).view(*shape[:-1], J)
+    return y[..., :J] if pad_j else y

@@ -33,8 +33,10 @@ def test_refusals():
 def test_plan():
     big = _lib.product_plan(32768, 4096, 2048, -1)
     assert big.forward_work_bytes == 0 and big.dbpart_bytes > 0
-    few = _lib.product_plan(64, 256, 8192, -1)             # one tile and a long sum: cut into parts
-    assert few.forward_work_bytes >= 2 * 4 * 64 * 256
+    few = _lib.product_plan(300, 256, 8192, -1)            # two tiles and a long sum: cut into parts
+    assert few.forward_work_bytes >= 2 * 4 * 300 * 256 and few.forward_waits
+    assert not _lib.product_plan(16, 8192, 8192, -1).forward_waits and not _lib.product_plan(256, 1024, 1024, -1).forward_waits
+    assert _lib.product_plan(257, 1024, 1024, -1).forward_waits and _lib.product_plan(17, 4096, 4096, -1).forward_waits
     tall = _lib.product_plan(9000, 24, 72, -1)             # dW has one tile and sums 9000 rows
     assert tall.backward_work_bytes >= 2 * 4 * 24 * 72
     lib, out = _lib.load(), _lib.ProductPlan()
@@ -47,7 +49,7 @@ def test_c_entries_refuse_before_any_launch():
     lib = _lib.load()
     f = lambda x=16, w=16, bias=16, y=16, act=1, M=8, J=8, I=8, err=16: lib.frnn_b200_product_forward(  # noqa: E731
         x, w, bias, 1, None, act, y, None, M, J, I, None, err, None)
-    assert f(x=None) == f(w=None) == f(y=None) == f(err=None, M=33) == f(act=4) == f(M=0) == f(x=8) == f(bias=4) == f(y=24) == -5
+    assert f(x=None) == f(w=None) == f(y=None) == f(err=None, M=300) == f(act=4) == f(M=0) == f(x=8) == f(bias=4) == f(y=24) == -5
     assert f(J=12) == f(I=4) == f(M=1 << 31) == -2
     g = lambda dy=16, z=16, x=16, w=16, act=1, dz=16, dx=16, part=16, I=8: lib.frnn_b200_product_backward(  # noqa: E731
         dy, z, x, w, act, dz, dx, 16, 16, 1, part, 8, 8, I, None, 16, None)

@@ -81,7 +81,8 @@ def check(got, ref, lim):
 
 # one row; less than, exactly and just over tiles of 128 and 256; K shorter than a stage and no multiple of one; more tiles than the
 # GPU holds; few tiles with a long K (cut into parts); features that are no multiple of eight
-SHAPES = [(1, 8, 8), (1, 768, 1536), (3, 40, 24), (16, 264, 72), (17, 64, 136), (31, 72, 40), (128, 64, 128), (129, 200, 136), (256, 64, 256),
+# (few rows take a kernel of their own: up to 8, 16, 32 and more to a CTA, K up to 1024 and longer, either side of where it ends)
+SHAPES = [(8, 2048, 264), (16, 1104, 40), (33, 520, 48), (70, 1032, 88), (256, 1024, 1024), (257, 1024, 1024), (260, 520, 1016), (17, 4096, 4096), (1, 8, 8), (1, 768, 1536), (3, 40, 24), (16, 264, 72), (17, 64, 136), (31, 72, 40), (128, 64, 128), (129, 200, 136), (256, 64, 256),
           (257, 520, 264), (300, 2048, 200), (1000, 768, 768), (5000, 128, 2504), (9000, 72, 24), (20, 1032, 16), (5, 33, 17), (130, 1001, 259)]
 
 
