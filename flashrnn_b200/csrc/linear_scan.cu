@@ -24,7 +24,7 @@ namespace frnn {
 
 namespace {
 
-constexpr int kGroup = 16;   // tiles of a group
+constexpr int kGroup = 8;    // tiles of a group
 constexpr unsigned long long kDefaultWaitNs = 2000000000ull;
 
 struct LinParams {
