@@ -28,12 +28,12 @@ constexpr int kThreads = 320;    // warps 0-7 epilogue, 8 TMA, 9 MMA
 constexpr int kEpiWarps = 8;
 constexpr int kKC = 64;          // k's per stage: 128 bytes of bf16, one swizzle row
 constexpr int kBufBytes = 4096;  // staging of a warp: two buffers of 32 rows x 128 bytes
+// All of an SM's shared memory, whatever a tile needs of it: no CTA of another kernel shares the SM, so that none holds tensor memory there
+// that this one's allocation, or its own peer on another SM, would have to wait for.
+constexpr int kSmem = 227 * 1024 - 512;
 // Stages of the ring: as many as fit beside the staging buffers. B along N comes in boxes of 64 columns, whole ones.
 __host__ __device__ constexpr int stage_bytes_of(int np, bool b_mn) { return 16384 + (b_mn ? (np / 2 + 63) / 64 * 8192 : np / 2 * 128); }
-__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (227 * 1024 - 2048 - kEpiWarps * 2 * kBufBytes) / stage_bytes_of(np, b_mn); }
-__host__ __device__ constexpr int smem_of(int np, bool b_mn) {
-  return stages_of(np, b_mn) * stage_bytes_of(np, b_mn) + kEpiWarps * 2 * kBufBytes + 1024;
-}
+__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (kSmem - 1024 - kEpiWarps * 2 * kBufBytes) / stage_bytes_of(np, b_mn); }
 constexpr uint64_t kLimit = 2000000000ull;
 
 struct ProductParams {
@@ -702,11 +702,11 @@ int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long lo
 template <bool A_MN, bool B_MN, int NP, int ACT>
 int launch_kernel(const ProductParams& p, const CUtensorMap (&maps)[6], cudaStream_t s) {
   const void* kern = reinterpret_cast<const void*>(product_kernel<A_MN, B_MN, NP, ACT>);
-  cudaError_t e = raise_limits(kern, smem_of(NP, B_MN), false);
+  cudaError_t e = raise_limits(kern, kSmem, false);
   if (e != cudaSuccess) return static_cast<int>(e);
   const long long pairs = sm_count() / 2;
   const unsigned grid = 2u * static_cast<unsigned>(p.n_units < pairs ? p.n_units : pairs);
-  product_kernel<A_MN, B_MN, NP, ACT><<<grid, kThreads, smem_of(NP, B_MN), s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5]);
+  product_kernel<A_MN, B_MN, NP, ACT><<<grid, kThreads, kSmem, s>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5]);
   return static_cast<int>(cudaGetLastError());
 }
 // The gradients' products have no epilogue.

@@ -38,8 +38,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """Contiguous and on the 16-byte boundary that the kernels' vector accesses need (a view may start anywhere)."""
-    if not t.is_contiguous():
-        return t.contiguous()
+    t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 

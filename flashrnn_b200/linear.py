@@ -79,7 +79,7 @@ class _LinearRecurrence(torch.autograd.Function):
         plan = _lib.linear_plan(ctx.function, B, T, N, D)
         d_hidden = wx.new_zeros((B, T, N, D)) if d_hidden is None else _dense(d_hidden)
         if d_last is not None:
-            d_last = d_last.contiguous()
+            d_last = _dense(d_last)
         d_wx, db = torch.empty_like(wx), torch.empty_like(bias)
         need = ctx.needs_input_grad
         d_initial = torch.empty_like(initial) if need[2] else None
@@ -178,6 +178,8 @@ def _run(wx, b, states, function, lengths, last_out, grad):
     if grad:
         return _LinearRecurrence.apply(wx, b, states, lengths, function)
     out = last_out
+    if out is not None and out.data_ptr() % 16:
+        out = None
     if out is not None and states is not None and states.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
         # a call of several steps may read `states` after other parts of `last` are written, and a step may where the two overlap
         # without being the same: a buffer in between
@@ -190,7 +192,4 @@ def _run(wx, b, states, function, lengths, last_out, grad):
 
 
 def _state(t: torch.Tensor) -> torch.Tensor:
-    """fp32 and contiguous"""
-    if t.dtype != torch.float32:
-        t = t.to(torch.float32)
-    return t if t.is_contiguous() else t.contiguous()
+    return _dense(t if t.dtype == torch.float32 else t.to(torch.float32))

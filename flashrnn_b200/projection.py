@@ -119,15 +119,28 @@ def _product_forward(x, weight, bias, residual, activation, keep: bool):
     return y, z
 
 
+def _whole_vectors(x, weight, bias, residual):
+    """The operands as the kernels take them: contiguous, aligned, features padded with zeros to multiples of 8."""
+    J, I = weight.shape
+    if I % 8 or J % 8:
+        pad, pad_i, pad_j = torch.nn.functional.pad, -I % 8, -J % 8
+        x, weight = pad(x, (0, pad_i)), pad(weight, (0, pad_i, 0, pad_j))
+        bias = None if bias is None else pad(bias, (0, pad_j))
+        residual = None if residual is None else pad(residual, (0, pad_j))
+    return _dense(x), _dense(weight), None if bias is None else _dense(bias), None if residual is None else _dense(residual)
+
+
 class _FusedProjection(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         need = ctx.needs_input_grad
+        J, I = weight.shape
+        x, weight, bias, residual = _whole_vectors(x, weight, bias, residual)
         y, z = _product_forward(x, weight, bias, residual, activation, need[0] or need[1] or need[2])
         ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, z)
-        ctx.activation, ctx.shapes = activation, (x.shape, weight.shape)
+        ctx.activation, ctx.shapes, ctx.features = activation, (x.shape, weight.shape), (J, I)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
+        return y[..., :J] if J % 8 else y
 
     @staticmethod
     def backward(ctx, dy):
@@ -146,10 +159,10 @@ class _FusedProjection(torch.autograd.Function):
         poll_errors()
         x, weight, z = ctx.saved_tensors
         x_shape, w_shape = ctx.shapes
-        J, I = w_shape
-        M = dy.numel() // J
+        features, (J, I) = ctx.features, w_shape
+        g = _dense(dy if features[0] == J else torch.nn.functional.pad(dy, (0, J - features[0])))
+        M = g.numel() // J
         plan = _lib.product_plan(M, J, I, dev.index)
-        g = _dense(dy)
         dx = g.new_empty(x_shape) if need_x else None
         dw = g.new_empty(w_shape) if need_w else None
         db = torch.empty(J, dtype=ctx.bias_dtype, device=dev) if need_b else None
@@ -169,6 +182,10 @@ class _FusedProjection(torch.autograd.Function):
         _launched(word, "frnn_b200_product_backward")   # earlier launches of the call have the word, whether a later one was accepted or not
         if rc:
             _lib.check(rc, "frnn_b200_product_backward")
+        if features != (J, I):
+            dx = None if dx is None else dx[..., :features[1]]
+            dw = None if dw is None else dw[:features[0], :features[1]]
+            db = None if db is None else db[:features[0]]
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -223,25 +240,13 @@ def _bf16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _run_product(x, weight, bias, activation, residual, grad: bool):
-    J, I = weight.shape
+    J = weight.shape[0]
     x, weight = _bf16(x), _bf16(weight)
     if residual is not None:
         residual = _bf16(residual)
     if bias is not None and bias.dtype != torch.bfloat16 and bias.dtype != torch.float32:
         bias = bias.to(torch.float32)
-    pad_i, pad_j = -I % 8, -J % 8
-    if pad_i or pad_j:
-        pad = torch.nn.functional.pad
-        x, weight = pad(x, (0, pad_i)), pad(weight, (0, pad_i, 0, pad_j))
-        bias = None if bias is None else pad(bias, (0, pad_j))
-        residual = None if residual is None else pad(residual, (0, pad_j))
-    x, weight = _dense(x), _dense(weight)
-    if bias is not None:
-        bias = _dense(bias)
-    if residual is not None:
-        residual = _dense(residual)
     if grad:
-        y = _FusedProjection.apply(x, weight, bias, residual, activation)
-    else:
-        y = _product_forward(x, weight, bias, residual, activation, False)[0]
-    return y[..., :J] if pad_j else y
+        return _FusedProjection.apply(x, weight, bias, residual, activation)
+    y = _product_forward(*_whole_vectors(x, weight, bias, residual), activation, False)[0]
+    return y[..., :J] if J % 8 else y

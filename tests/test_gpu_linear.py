@@ -194,6 +194,27 @@ def test_strides_offsets_and_other_types(cuda_device):
         g.float().sum().backward()
 
 
+@pytest.mark.parametrize("shape", [(3, 140, 2, 20), (2, 5, 1, 24), (500, 20, 1, 140)], ids=str)
+def test_every_tensor_may_start_anywhere(shape, cuda_device):
+    """Contiguous views that start four bytes behind a vector's boundary."""
+    from flashrnn_b200 import flashrnn_linear
+
+    def moved(t):
+        out = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view_as(t)
+        assert out.data_ptr() % 8 and out.is_contiguous()
+        return out.copy_(t)
+
+    wx, b, s, n, dh, dl = make("leaky", *shape, F32, 7, cuda_device, lengths="ragged")
+    want = step("leaky", wx, b, s, n, dh, dl)
+    got = step("leaky", *(moved(t) for t in (wx, b, s, n, dh, dl)))
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    last, first = moved(s), moved(s)
+    with torch.no_grad():
+        assert flashrnn_linear(wx, b, first, "leaky", n, last_out=last)[1] is last and torch.equal(last, want["last"])
+        flashrnn_linear(wx, b, first, "leaky", n, last_out=first)
+    assert torch.equal(first, want["last"])
+
+
 @pytest.mark.parametrize("T", [1, 60, 400])
 def test_last_out_in_place_and_on_another_stream(T, cuda_device):
     from flashrnn_b200 import flashrnn_linear

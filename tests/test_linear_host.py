@@ -50,16 +50,19 @@ def test_plan():
     assert p.exchange_bytes >= 8 * 8 * 768 * 8
     one = _lib.linear_plan("lstm", 1, _lib.linear_plan("lstm", 1, 1, 1, 1).tile_steps, 1, 7)
     assert (one.gates, one.tiles, one.exchange_bytes, one.starts_bytes, one.dbpart_bytes) == (4, 1, 0, 0, 0)
+    many = _lib.linear_plan("leaky", 4096, 2 ** 20, 8, 128)        # sizes past 32 bits
+    assert many.starts_bytes == 4 * 4096 * (2 ** 17 - 1) * 1024 and many.dbpart_bytes == 4 * 4096 * 2 * 1024
     lib = _lib.load()
-    for a, rc in (((2, 1, 1, 1, 1), -1), ((0, 0, 1, 1, 1), -5), ((0, 1, 1, 1, 0), -5), ((0, 1, 1, 2 ** 16, 2 ** 16), -2), ((1, 2 ** 30, 2 ** 10, 1, 1), -2)):
+    for a, rc in (((2, 1, 1, 1, 1), -1), ((0, 0, 1, 1, 1), -5), ((0, 1, 1, 1, 0), -5), ((0, 1, 1, 2 ** 16, 2 ** 16), -2), ((1, 2 ** 30, 2 ** 10, 1, 1), -2), ((1, 1, 2 ** 31 - 1, 1, 1), -2)):
         assert lib.frnn_b200_linear_plan(*a, one) == rc, a
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="calls with pointers to nothing")
 def test_c_entries_refuse_before_any_launch():
     lib = _lib.load()
-    f = lambda wx=16, bias=16, hidden=16, last=16, exchange=16, err=16, T=300: lib.frnn_b200_linear_forward(  # noqa: E731
-        0, wx, 1, bias, None, None, hidden, last, None, exchange, 1, T, 1, 8, 0, err, None)
+    f = lambda wx=16, bias=16, hidden=16, last=16, exchange=16, err=16, T=300, first=None: lib.frnn_b200_linear_forward(  # noqa: E731
+        0, wx, 1, bias, first, None, hidden, last, None, exchange, 1, T, 1, 8, 0, err, None)
+    assert f(bias=4) == f(last=8) == f(first=20) == -5 and f(T=2 ** 31 - 1) == -2
     assert f(wx=None) == f(bias=None) == f(hidden=None) == f(last=None) == f(wx=24) == f(hidden=8) == -5
     assert f(exchange=None) == f(err=None) == f(exchange=24) == f(T=0) == -5
     g = lambda starts=16, part=16, dwx=16, dh=16: lib.frnn_b200_linear_backward(  # noqa: E731
