@@ -27,13 +27,13 @@ namespace {
 constexpr int kThreads = 320;    // warps 0-7 epilogue, 8 TMA, 9 MMA
 constexpr int kEpiWarps = 8;
 constexpr int kKC = 64;          // k's per stage: 128 bytes of bf16, one swizzle row
-constexpr int kBufBytes = 4096;  // staging of a warp: two buffers of 32 rows x 128 bytes
+constexpr int kBufBytes = 2048;  // staging of a warp: four buffers of 32 rows x 64 bytes, a piece of 32 columns
 // All of an SM's shared memory, whatever a tile needs of it: no CTA of another kernel shares the SM, so that none holds tensor memory there
 // that this one's allocation, or its own peer on another SM, would have to wait for.
 constexpr int kSmem = 227 * 1024 - 512;
 // Stages of the ring: as many as fit beside the staging buffers. B along N comes in boxes of 64 columns, whole ones.
 __host__ __device__ constexpr int stage_bytes_of(int np, bool b_mn) { return 16384 + (b_mn ? (np / 2 + 63) / 64 * 8192 : np / 2 * 128); }
-__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (kSmem - 1024 - kEpiWarps * 2 * kBufBytes) / stage_bytes_of(np, b_mn); }
+__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (kSmem - 1024 - kEpiWarps * 4 * kBufBytes) / stage_bytes_of(np, b_mn); }
 constexpr uint64_t kLimit = 2000000000ull;
 
 struct ProductParams {
@@ -205,7 +205,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
   extern __shared__ uint8_t smem_raw[];
   constexpr int kStages = stages_of(NP, B_MN);
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2], s_done;
-  __shared__ __align__(8) uint64_t s_res[kEpiWarps][2];
+  __shared__ __align__(8) uint64_t s_res[kEpiWarps][4];
   __shared__ uint32_t s_tmem_base;
   constexpr int NH = NP / 2;  // rows of B in each CTA
   constexpr uint32_t kStageBytes = stage_bytes_of(NP, B_MN), kCols = NP > 128 ? 512u : 2u * NP;
@@ -226,7 +226,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       mbar_init(smem_u32(&s_acc_empty[a]), 2 * kEpiWarps);  // the epilogue warps of both CTAs, in the even one
     }
     for (int w = 0; w < kEpiWarps; ++w)
-      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
+      for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
     mbar_init(smem_u32(&s_done), 1);
     fence_mbar_init();
   }
@@ -349,34 +349,31 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
     }
   } else {
     const int q = warp & 3, half = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; columns
-    constexpr int CW = 64;            // columns of a piece: 128 bytes
-    constexpr int kPieces = NP / CW;  // of the tile, in turn to the two warps of a quarter
-    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 2u * kBufBytes;
-    const uint32_t my_row = static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
-    // Without z the pieces take the two buffers in turn; with it z goes through the first, y through the second. The residual's
-    // piece is loaded into the buffer that y leaves from.
+    constexpr int CW = 32;            // columns of a piece
+    constexpr int kPieces = NP / CW;  // of the tile, in turn to the two warps of a quarter: up to four for each
+    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 4u * kBufBytes;
+    const uint32_t my_row = static_cast<uint32_t>(lane) * 64u, sw = static_cast<uint32_t>((lane >> 1) & 3);  // TMA's 64-byte swizzle
+    // Without z the pieces take the four buffers in turn; with it z has the first two and y the others. The residual's piece is loaded
+    // into the buffer that y leaves from.
     const bool z_too = ACT != FRNN_ACT_NONE && p.has_z;
     uint32_t li = 0, used = 0, res_phase = 0;  // used: pieces staged so far; res_phase: a bit per buffer
-    auto ask_residual = [&](uint32_t bi, int j, int m) {
-      const uint32_t bar = smem_u32(&s_res[warp][bi]);
+    auto y_slot = [&](uint32_t n) { return z_too ? 2u + (n & 1u) : n & 3u; };
+    auto ask_residual = [&](uint32_t slot, int j, int m) {
+      const uint32_t bar = smem_u32(&s_res[warp][slot]);
       mbar_arrive_expect_tx(bar, kBufBytes);
-      tma_load_2d(buf0 + bi * kBufBytes, &res_map, bar, j, m);
+      tma_load_2d(buf0 + slot * kBufBytes, &res_map, bar, j, m);
     };
     for (long long t = pair; t < p.n_units; t += pairs, ++li) {
       const Tile tile = tile_at(t);
       const uint32_t a = li & 1u;
       const int mw = tile.m0 + 128 * cta + 32 * q, j0 = tile.n0;
       const bool any = mw < p.M, part = tile.row0 >= 0;  // warp-uniform
-      if (p.has_residual && any && !part && lane == 0) {   // while the tensor cores work
+      if (p.has_residual && any && !part && lane == 0) {   // while the tensor cores work: as many pieces as there are buffers
         tma_store_wait_read<0>();
-        if (z_too) {
-          if (j0 + half * CW < p.N) ask_residual(1, j0 + half * CW, mw);
-        } else {
-#pragma unroll
-          for (int i = 0; i < kPieces / 2 + kPieces % 2; ++i) {
-            const int piece = half + 2 * i;
-            if (piece < kPieces && j0 + piece * CW < p.N) ask_residual((used + i) & 1u, j0 + piece * CW, mw);
-          }
+        const int ahead = z_too ? 2 : 4;
+        for (int n = 0; n < ahead; ++n) {
+          const int piece = half + 2 * n;
+          if (piece < kPieces && j0 + piece * CW < p.N) ask_residual(y_slot(used + n), j0 + piece * CW, mw);
         }
       }
       const bool have = mbar_wait_warp<false>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag);
@@ -399,14 +396,14 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
           tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * 32), v);
           tmem_ld_wait();
           if (i + 2 >= kParts) release();
-          const uint32_t buf = buf0 + (used & 1u) * kBufBytes + my_row;
+          const uint32_t buf = buf0 + (used & 1u) * 2u * kBufBytes + static_cast<uint32_t>(lane) * 128u;
           ++used;
           if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t w[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
-            st_shared_v4(buf + ((k ^ sw) << 4), w);
+            st_shared_v4(buf + ((k ^ (lane & 7)) << 4), w);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -419,58 +416,60 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       }
 #pragma unroll 1
       for (int i = half; i < kPieces; i += 2) {
-        const int c = a * NP + i * CW, j = j0 + i * CW;
+        const int j = j0 + i * CW;
         float v[CW];
-        tmem_ld_x32(tmem_addr(tbase, 32 * q, c), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld_x32(tmem_addr(tbase, 32 * q, c + 32), *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * CW), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
         tmem_ld_wait();
         if (i + 2 >= kPieces) release();
         if (!any || j >= p.N) continue;
-        const uint32_t bi = z_too ? 1u : used & 1u, buf = buf0 + bi * kBufBytes + my_row;
+        const uint32_t slot = y_slot(used), y_at = buf0 + slot * kBufBytes, z_at = buf0 + (used & 1u) * kBufBytes;
         ++used;
         if (p.bias != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
+          for (int k = 0; k < 4; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
         }
-        if (lane == 0) {
-          if (z_too) tma_store_wait_read<0>();
-          else if (!p.has_residual) tma_store_wait_read<1>();
+        if (lane == 0) {  // the stores that read these buffers two or four pieces ago; with a residual and no z: before it was asked for
+          if (z_too) tma_store_wait_read<1>();
+          else if (!p.has_residual) tma_store_wait_read<3>();
         }
         __syncwarp();
         if (z_too) {
-          if (p.has_residual && i >= 2 && lane == 0) ask_residual(1, j, mw);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 4; ++k) {
             uint32_t w[4];
             keep_slope<ACT>(&v[8 * k], w);
-            st_shared_v4(buf0 + my_row + ((k ^ sw) << 4), w);
+            st_shared_v4(z_at + my_row + ((k ^ sw) << 4), w);
           }
         }
         act_row<ACT>(v);
         if (p.has_residual) {
-          if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][bi]), (res_phase >> bi) & 1u, kLimit, abort_flag)) {
+          if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][slot]), (res_phase >> slot) & 1u, kLimit, abort_flag)) {
             if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
           }
-          res_phase ^= 1u << bi;
+          res_phase ^= 1u << slot;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 4; ++k) {
             uint32_t w[4];
-            ld_shared_v4(buf + ((k ^ sw) << 4), w);
+            ld_shared_v4(y_at + my_row + ((k ^ sw) << 4), w);
             add_bf16(w, &v[8 * k]);
           }
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
           const float* f = &v[8 * k];
           const uint32_t w[4] = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
-          st_shared_v4(buf + ((k ^ sw) << 4), w);
+          st_shared_v4(y_at + my_row + ((k ^ sw) << 4), w);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_2d(&out_map, buf, j, mw);
-          if (z_too) tma_store_2d(&z_map, buf0, j, mw);
+          tma_store_2d(&out_map, y_at, j, mw);
+          if (z_too) tma_store_2d(&z_map, z_at, j, mw);
           tma_store_commit();
+          if (z_too && p.has_residual && i >= 2 && i + 2 < kPieces && j + 2 * CW < p.N) {  // the other buffer's store is behind this one's
+            tma_store_wait_read<1>();
+            ask_residual(y_slot(used), j + 2 * CW, mw);
+          }
         }
       }
     }
@@ -693,10 +692,11 @@ long long work_bytes(long long M, long long N, long long K) {
   return 4 * c.rest * c.parts * 256 * c.np;
 }
 
+// Rows of `cols` values, boxes whose rows fill the span of the swizzle (64 or 128 bytes).
 int map_2d(CUtensorMap* map, const void* base, int elem, long long cols, long long rows, uint32_t box_cols, uint32_t box_rows) {
-  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)}, strides[1] = {static_cast<uint64_t>(cols) * elem};
   const uint32_t box[2] = {box_cols, box_rows};
-  return make_tensor_map(map, base, elem, 2, dims, box, true);
+  return make_tensor_map_strided(map, base, elem, 2, dims, strides, box, static_cast<int>(box_cols) * elem);
 }
 
 template <bool A_MN, bool B_MN, int NP, int ACT>
@@ -736,9 +736,9 @@ int product_launch(ProductParams p, const void* A, const void* B, long long M, l
   const uint32_t half = static_cast<uint32_t>(cut.np / 2);
   int rc = A_MN ? map_2d(&maps[0], A, 2, M, K, 64, kKC) : map_2d(&maps[0], A, 2, K, M, kKC, 128);
   if (rc == 0) rc = B_MN ? map_2d(&maps[1], B, 2, N, K, 64, kKC) : map_2d(&maps[1], B, 2, K, N, kKC, half);
-  if (rc == 0) rc = map_2d(&maps[2], out, 2, N, M, 64, 32);
-  if (rc == 0 && residual != nullptr) rc = map_2d(&maps[3], residual, 2, N, M, 64, 32);
-  if (rc == 0 && z != nullptr) rc = map_2d(&maps[4], z, 2, N, M, 64, 32);
+  if (rc == 0) rc = map_2d(&maps[2], out, 2, N, M, 32, 32);
+  if (rc == 0 && residual != nullptr) rc = map_2d(&maps[3], residual, 2, N, M, 32, 32);
+  if (rc == 0 && z != nullptr) rc = map_2d(&maps[4], z, 2, N, M, 32, 32);
   if (rc == 0 && cut.rest > 0) rc = map_2d(&maps[5], work, 4, cut.np, cut.rest * cut.parts * 256, 32, 32);
   if (rc != 0) return rc;
   if (residual == nullptr) maps[3] = maps[2];
