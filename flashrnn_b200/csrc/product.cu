@@ -24,16 +24,16 @@ namespace frnn {
 
 namespace {
 
-constexpr int kThreads = 320;    // warps 0-7 epilogue, 8 TMA, 9 MMA
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;                     // four to each quarter of the tensor memory's lanes
+constexpr int kThreads = (kEpiWarps + 2) * 32;    // then TMA, MMA
 constexpr int kKC = 64;          // k's per stage: 128 bytes of bf16, one swizzle row
-constexpr int kBufBytes = 2048;  // staging of a warp: four buffers of 32 rows x 64 bytes, a piece of 32 columns
+constexpr int kBufBytes = 2048;  // staging of a warp: two buffers of 32 rows x 64 bytes, a piece of 32 columns
 // All of an SM's shared memory, whatever a tile needs of it: no CTA of another kernel shares the SM, so that none holds tensor memory there
 // that this one's allocation, or its own peer on another SM, would have to wait for.
 constexpr int kSmem = 227 * 1024 - 512;
 // Stages of the ring: as many as fit beside the staging buffers. B along N comes in boxes of 64 columns, whole ones.
 __host__ __device__ constexpr int stage_bytes_of(int np, bool b_mn) { return 16384 + (b_mn ? (np / 2 + 63) / 64 * 8192 : np / 2 * 128); }
-__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (kSmem - 1024 - kEpiWarps * 4 * kBufBytes) / stage_bytes_of(np, b_mn); }
+__host__ __device__ constexpr int stages_of(int np, bool b_mn) { return (kSmem - 1024 - kEpiWarps * 2 * kBufBytes) / stage_bytes_of(np, b_mn); }
 constexpr uint64_t kLimit = 2000000000ull;
 
 struct ProductParams {
@@ -173,6 +173,9 @@ __device__ __forceinline__ void keep_slope(const float* v, uint32_t (&w)[4]) {
     else w[i] = pack_half2(a, b);
   }
 }
+__device__ __forceinline__ float load_bias(const ProductParams& p, int j) {
+  return p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[j]) : __ldg(static_cast<const float*>(p.bias) + j);
+}
 // v[i] += bias[j + i], eight columns of a row of N (a multiple of eight)
 __device__ __forceinline__ void add_bias(const ProductParams& p, int j, float* v) {
   if (j >= p.N) return;
@@ -205,7 +208,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
   extern __shared__ uint8_t smem_raw[];
   constexpr int kStages = stages_of(NP, B_MN);
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2], s_done;
-  __shared__ __align__(8) uint64_t s_res[kEpiWarps][4];
+  __shared__ __align__(8) uint64_t s_res[kEpiWarps][2];
   __shared__ uint32_t s_tmem_base;
   constexpr int NH = NP / 2;  // rows of B in each CTA
   constexpr uint32_t kStageBytes = stage_bytes_of(NP, B_MN), kCols = NP > 128 ? 512u : 2u * NP;
@@ -226,18 +229,18 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       mbar_init(smem_u32(&s_acc_empty[a]), 2 * kEpiWarps);  // the epilogue warps of both CTAs, in the even one
     }
     for (int w = 0; w < kEpiWarps; ++w)
-      for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
+      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_res[w][i]), 1);
     mbar_init(smem_u32(&s_done), 1);
     fence_mbar_init();
   }
-  if (warp == 7 && lane == 0) {
+  if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&a_map);
     tma_prefetch_desc(&b_map);
     tma_prefetch_desc(&out_map);
     if (p.has_residual) tma_prefetch_desc(&res_map);
     if (p.has_z) tma_prefetch_desc(&z_map);
   }
-  if (warp == 9) tmem_alloc_pair(smem_u32(&s_tmem_base), kCols);
+  if (warp == kEpiWarps + 1) tmem_alloc_pair(smem_u32(&s_tmem_base), kCols);
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();
@@ -263,7 +266,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
     return r;
   };
 
-  if (warp == 8) {
+  if (warp == kEpiWarps) {
     if (lane == 0) {
       uint32_t s = 0, round = 0;
       bool dead = false;
@@ -307,7 +310,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kEpiWarps + 1) {
     if (lane == 0 && cta == 0) {
       const uint32_t idesc = umma_idesc_bf16(256, NP, A_MN, B_MN);
       uint32_t s = 0, round = 0, li = 0;
@@ -348,16 +351,18 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       mbar_wait_bounded<false, true>(smem_u32(&s_done), 0, kLimit, nullptr);
     }
   } else {
-    const int q = warp & 3, half = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; columns
-    constexpr int CW = 32;            // columns of a piece
-    constexpr int kPieces = NP / CW;  // of the tile, in turn to the two warps of a quarter: up to four for each
-    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 4u * kBufBytes;
+    const int q = warp & 3, first = warp >> 2;  // quarter of the tensor memory's lanes that this warp may read; its first piece
+    constexpr int CW = 32;             // columns of a piece
+    constexpr int kPieces = NP / CW;   // of the tile, in turn to the four warps of a quarter: one or two for each
+    constexpr int kTurn = kEpiWarps / 4;
+    const uint32_t buf0 = staging + static_cast<uint32_t>(warp) * 2u * kBufBytes;
     const uint32_t my_row = static_cast<uint32_t>(lane) * 64u, sw = static_cast<uint32_t>((lane >> 1) & 3);  // TMA's 64-byte swizzle
-    // Without z the pieces take the four buffers in turn; with it z has the first two and y the others. The residual's piece is loaded
-    // into the buffer that y leaves from.
+    // Without z the pieces take the two buffers in turn; with it z has the first and y the second. The residual's piece is loaded into
+    // the buffer that y leaves from. What takes time here is latency, not arithmetic: hence four warps to a scheduler, and everything
+    // that does not need the accumulator is asked for before it is waited for.
     const bool z_too = ACT != FRNN_ACT_NONE && p.has_z;
     uint32_t li = 0, used = 0, res_phase = 0;  // used: pieces staged so far; res_phase: a bit per buffer
-    auto y_slot = [&](uint32_t n) { return z_too ? 2u + (n & 1u) : n & 3u; };
+    auto y_slot = [&](uint32_t n) { return z_too ? 1u : n & 1u; };
     auto ask_residual = [&](uint32_t slot, int j, int m) {
       const uint32_t bar = smem_u32(&s_res[warp][slot]);
       mbar_arrive_expect_tx(bar, kBufBytes);
@@ -370,13 +375,20 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       const bool any = mw < p.M, part = tile.row0 >= 0;  // warp-uniform
       if (p.has_residual && any && !part && lane == 0) {   // while the tensor cores work: as many pieces as there are buffers
         tma_store_wait_read<0>();
-        const int ahead = z_too ? 2 : 4;
+        const int ahead = z_too ? 1 : 2;
         for (int n = 0; n < ahead; ++n) {
-          const int piece = half + 2 * n;
+          const int piece = first + kTurn * n;
           if (piece < kPieces && j0 + piece * CW < p.N) ask_residual(y_slot(used + n), j0 + piece * CW, mw);
         }
       }
-      const bool have = mbar_wait_warp<false>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag);
+      float bias[(kPieces + kTurn - 1) / kTurn];  // of this lane's column of each piece
+#pragma unroll
+      for (int n = 0; n < (kPieces + kTurn - 1) / kTurn; ++n) {
+        const int j = j0 + (first + kTurn * n) * CW + lane;
+        bias[n] = p.bias != nullptr && !part && j < p.N ? load_bias(p, j) : 0.0f;
+      }
+      // parked, not polled: sixteen polling warps take issue slots and power from a long sum's tensor cores
+      const bool have = __all_sync(0xffffffffu, mbar_wait_bounded<false, false>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag));
       if (!have) {
         if (lane == 0) atomicCAS(p.err, 0, kErrWaitMma);
         break;
@@ -388,17 +400,14 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s_acc_empty[a]), 0));
       };
       if (part) {
-        constexpr int kParts = NP / 32;  // pieces of 32 columns in fp32
-        if (lane == 0) tma_store_wait_read<0>();
 #pragma unroll 1
-        for (int i = half; i < kParts; i += 2) {
+        for (int i = first; i < kPieces; i += kTurn) {  // 32 columns of fp32 take both buffers
           uint32_t v[32];
-          tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * 32), v);
+          tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * CW), v);
           tmem_ld_wait();
-          if (i + 2 >= kParts) release();
-          const uint32_t buf = buf0 + (used & 1u) * 2u * kBufBytes + static_cast<uint32_t>(lane) * 128u;
-          ++used;
-          if (lane == 0) tma_store_wait_read<1>();  // the store that read this buffer two pieces ago
+          if (i + kTurn >= kPieces) release();
+          const uint32_t buf = buf0 + static_cast<uint32_t>(lane) * 128u;
+          if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -408,31 +417,33 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&work_map, buf, i * 32, tile.row0 + 128 * cta + 32 * q);
+            tma_store_2d(&work_map, buf, i * CW, tile.row0 + 128 * cta + 32 * q);
             tma_store_commit();
           }
         }
         continue;
       }
-#pragma unroll 1
-      for (int i = half; i < kPieces; i += 2) {
-        const int j = j0 + i * CW;
+#pragma unroll
+      for (int n = 0; n < (kPieces + kTurn - 1) / kTurn; ++n) {
+        const int i = first + kTurn * n, j = j0 + i * CW;
+        if (i >= kPieces) break;
         float v[CW];
         tmem_ld_x32(tmem_addr(tbase, 32 * q, a * NP + i * CW), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
         tmem_ld_wait();
-        if (i + 2 >= kPieces) release();
+        if (i + kTurn >= kPieces) release();
         if (!any || j >= p.N) continue;
-        const uint32_t slot = y_slot(used), y_at = buf0 + slot * kBufBytes, z_at = buf0 + (used & 1u) * kBufBytes;
+        const uint32_t slot = y_slot(used), y_at = buf0 + slot * kBufBytes, z_at = buf0;
         ++used;
         if (p.bias != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) add_bias(p, j + 8 * k, &v[8 * k]);
+          for (int k = 0; k < CW; k += 2) add2(v[k], v[k + 1], __shfl_sync(0xffffffffu, bias[n], k), __shfl_sync(0xffffffffu, bias[n], k + 1));
         }
-        if (lane == 0) {  // the stores that read these buffers two or four pieces ago; with a residual and no z: before it was asked for
-          if (z_too) tma_store_wait_read<1>();
-          else if (!p.has_residual) tma_store_wait_read<3>();
+        if (lane == 0) {  // the stores that read these buffers; with a residual and no z: before it was asked for
+          if (z_too) tma_store_wait_read<0>();
+          else if (!p.has_residual) tma_store_wait_read<1>();
         }
         __syncwarp();
+        if (z_too && p.has_residual && n > 0 && lane == 0) ask_residual(slot, j, mw);
         if (z_too) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -466,10 +477,6 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
           tma_store_2d(&out_map, y_at, j, mw);
           if (z_too) tma_store_2d(&z_map, z_at, j, mw);
           tma_store_commit();
-          if (z_too && p.has_residual && i >= 2 && i + 2 < kPieces && j + 2 * CW < p.N) {  // the other buffer's store is behind this one's
-            tma_store_wait_read<1>();
-            ask_residual(y_slot(used), j + 2 * CW, mw);
-          }
         }
       }
     }
@@ -478,7 +485,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();  // the other CTA's operands, barriers and tensor memory are in use until here
-  if (warp == 9) tmem_dealloc_pair(tbase, kCols);
+  if (warp == kEpiWarps + 1) tmem_dealloc_pair(tbase, kCols);
 }
 
 // out = epilogue(sum over the parts of a tile), eight columns of a row to a thread; work [tile][part][256][np].
