@@ -332,7 +332,7 @@ struct Fetched {
 };
 // ... and they are composed in order with the state at the start of the group, which the last tile of the group before hands out.
 template <int CW>
-__device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x, int k, int channel, const float2 (*s_prev)[CW], float first,
+__device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x, int k, bool mute, int channel, const float2 (*s_prev)[CW], float first,
                                            float a, float h) {
   const int group = k / kGroup, at = k % kGroup;
   float ra = 1.0f, rh = 0.0f;
@@ -350,25 +350,33 @@ __device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x
     first = __uint_as_float(v);
   }
   const float carry = fmaf(ra, first, rh);
-  if (k + 1 < p.n_tiles && at == kGroup - 1)
+  if (k + 1 < p.n_tiles && at == kGroup - 1 && !mute)
     st_relaxed_gpu_u32(x.states + (static_cast<long long>(group + 1) * CW + channel) * 4, xg_clean(__float_as_uint(fmaf(a, carry, h))));
   return carry;
 }
 
 // The tile of this CTA, from the counter where tiles wait on one another: k, row, b, channel block, and the row's length. One
 // thread divides for all.
-struct TileId { int k, row, b, cg, len; };
+struct TileId { int k, row, b, cg, len, mute; };
 __device__ __forceinline__ TileId lin_tile(const LinParams& p, TileId* shared) {
   if (threadIdx.x == 0) {
     int id = static_cast<int>(blockIdx.x);
-    if (p.n_tiles > 1) id = atomicAdd(reinterpret_cast<int*>(p.exchange), 1) + 1;  // it starts at -1
     TileId t;
+    t.mute = 0;
+    int from = 0;
+    if (p.n_tiles > 1) {
+      // test hook: with err[4] set, tiles from err[5] on in the order of the scan hand nothing out
+      t.mute = static_cast<volatile int*>(p.err)[4];
+      from = static_cast<volatile int*>(p.err)[5];
+      id = atomicAdd(reinterpret_cast<int*>(p.exchange), 1) + 1;  // it starts at -1
+    }
     const int rows = p.B * p.n_cg;
     t.k = id / rows;
     t.row = id - t.k * rows;
     t.b = t.row / p.n_cg;
     t.cg = t.row - t.b * p.n_cg;
     t.len = p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + t.b), 0), p.T);
+    if (t.k < from) t.mute = 0;
     *shared = t;
   }
   __syncthreads();
@@ -386,7 +394,7 @@ struct Shared {
 // (null: zeros) is what the row starts from; done(state, channel, carry, end) is called per channel with its place in [B][ND], what
 // the tile starts from and what it ends with. The maps are in place and a barrier is behind them.
 template <int CW, int NW, bool REVERSE, typename F>
-__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, const float* first, Shared<CW, NW>& s, Fetched<CW, NW>& got,
+__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, bool mute, const float* first, Shared<CW, NW>& s, Fetched<CW, NW>& got,
                                          F done) {
   const int nw = blockDim.x >> 5, b = row / p.n_cg, c0 = (row % p.n_cg) * CW, n_channels = min(CW, p.ND - c0);
   const Exchange x(p, row, CW);
@@ -400,7 +408,7 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, con
       h = fmaf(wa, h, wh);
       a *= wa;
     }
-    if (p.n_tiles > 1) lin_publish(p, x, k, c, CW, a, h);
+    if (p.n_tiles > 1 && !mute) lin_publish(p, x, k, c, CW, a, h);
   }
   if (p.n_tiles > 1) {
     got.put(p, s.prev);
@@ -409,7 +417,7 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, con
   if (c < n_channels) {
     const long long state = static_cast<long long>(b) * p.ND + c0 + c;
     float carry = first != nullptr && k < kGroup ? __ldg(first + state) : 0.0f;
-    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, c, s.prev, carry, a, h);
+    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, mute, c, s.prev, carry, a, h);
     done(state, c0 + c, carry, fmaf(a, carry, h));
 #pragma unroll 4
     for (int i = 0; i < nw; ++i) {
@@ -425,7 +433,7 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, con
 template <int VEC, int L, int TILE>
 struct Place {
   int k, row, b, c0, chl, ch, warp, span, t0, len;
-  bool ok, whole;  // ok: the channels exist; whole: and so do all steps of the warp
+  bool ok, whole, mute;  // ok: the channels exist; whole: and so do all steps of the warp
   __device__ __forceinline__ Place(const LinParams& p, const TileId& id, bool reverse) {
     using W = Lanes<VEC>;
     const int lane = threadIdx.x & 31;
@@ -440,6 +448,7 @@ struct Place {
     t0 = k * TILE + (warp * W::kSpans + span) * L;
     ok = ch < p.ND;
     len = id.len;
+    mute = id.mute != 0;
     whole = k * TILE + (warp + 1) * W::kSpans * L <= len && c0 + W::kChannels <= p.ND;
   }
   __device__ __forceinline__ bool valid(int l) const { return ok && t0 + l < len; }
@@ -555,7 +564,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   }
   join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
-  lin_join<CW, NW, false>(p, at.row, at.k, p.initial, s, got, [&](long long state, int channel, float carry, float end) {
+  lin_join<CW, NW, false>(p, at.row, at.k, at.mute, p.initial, s, got, [&](long long state, int channel, float carry, float end) {
     if (p.starts != nullptr && at.k > 0) p.starts[(static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + channel] = carry;
     if (at.k == p.n_tiles - 1) p.last[state] = end;
   });
@@ -722,7 +731,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   }
   join_spans<VEC, true>(at.span, A, E, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
-  lin_join<CW, NW, true>(p, at.row, kr, p.d_last, s, got, [&](long long state, int, float, float end) {
+  lin_join<CW, NW, true>(p, at.row, kr, at.mute, p.d_last, s, got, [&](long long state, int, float, float end) {
     if (at.k == 0 && p.d_initial != nullptr) p.d_initial[state] = end;
   });
   E = fma_(A, at.ok ? load_<VEC>(&s.start[at.warp][at.chl]) : splat<VEC>(0.0f), E);
@@ -787,6 +796,10 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
 // Many channels: there is no need to cut time. A thread walks its two channels (one, where ND is odd) through the whole sequence, the
 // next steps' loads in flight while it computes; no exchange, a third of the instructions of a tile. The states it keeps for the
 // backward pass are kWalkSteps apart: what the backward walk recomputes between two of them stays in registers.
+// A step takes 80 - 100 ns however many threads there are, until the memory is full, so it depends on the channels B N D who is faster;
+// walk against tile, forward + backward, us: leaky bf16 131072 x T2048 309 + 509, 494 + 813; 65536 220 + 354, 266 + 413; 32768 x T4096 355 +
+// 564, 251 + 419; lstm 131072 773 + 1315, 869 + 1648; 65536 468 + 746, 423 + 802. Channels that are no multiple of four have slower tiles: 48960 x
+// T512 52 + 87, 62 + 114. Up to 16 steps there is nothing to cut: 4 x 1 x 768 2.5 us, 4.9 in a tile.
 constexpr int kWalkSteps = 8, kWalkThreads = 64;
 constexpr long long kWalkChannels = 65536, kWalkOddChannels = 32768;
 

@@ -122,6 +122,8 @@ def flashrnn_linear(Wx: torch.Tensor, b: torch.Tensor, states: Optional[torch.Te
     behind a row's length leave its state alone, so ``last`` is the state at its end, and their hidden states and gradients are
     zeros, whatever Wx holds there.
 
+    A state that becomes infinite turns into a NaN one step later, in its channel only (its decay is infinity minus infinity).
+
     ``last_out`` (without gradients only) is written and returned as ``last``; it may be ``states`` itself, which a captured
     decoding step then updates in place.
     """

@@ -235,7 +235,8 @@ typedef struct frnn_b200_linear_plan {
 int frnn_b200_linear_plan(int function, int B, int T, int N, int D, frnn_b200_linear_plan_t* out);
 
 /* starts: NULL for inference, or where plan.starts_bytes is 0. With one tile `last` may be `initial`. A wait that runs out
- * (exchange_bytes > 0) is reported through err as 106. */
+ * (exchange_bytes > 0) is reported through err as 106. Test hook for that: with err[4] = 1 the tiles from err[5] on, in the order of the
+ * scan, hand nothing to those behind them. */
 int frnn_b200_linear_forward(int function, const void* wx, int wx_bf16, const float* bias, const float* initial, const int* lengths,
                              void* hidden, float* last, float* starts, void* exchange, int B, int T, int N, int D, int wait_limit_ms,
                              int* err, void* stream);

@@ -288,6 +288,44 @@ def test_captured_decoding_and_training(cuda_device):
     del graph
 
 
+@pytest.mark.parametrize("mute", [0, 1, 7])
+@pytest.mark.parametrize("backward", [False, True], ids=["forward", "backward"])
+def test_a_wait_that_runs_out_is_reported(backward, mute, cuda_device):
+    """Tiles that hand nothing out (7: the state between two groups): the call ends within its limit, says so, and the next one is right."""
+    from flashrnn_b200 import _lib
+
+    B, T, N, D = 2, 1300, 1, 64
+    wx, b, s, _, dh, dl = make("leaky", B, T, N, D, B16, 14, cuda_device)
+    want = step("leaky", wx, b, s, None, dh, dl)
+    lib, plan = _lib.load(), _lib.linear_plan("leaky", B, T, N, D)
+    assert plan.tiles > 9
+    exchange, err = torch.empty(plan.exchange_bytes, dtype=torch.uint8, device=cuda_device), torch.zeros(32, dtype=torch.int32, device=cuda_device)
+    starts, part = torch.zeros(plan.starts_bytes // 4, device=cuda_device), torch.zeros(plan.dbpart_bytes // 4, device=cuda_device)
+    out, last, db, d_init = torch.empty_like(dh), torch.empty_like(s), torch.empty_like(b), torch.empty_like(s)
+    d_wx = torch.empty_like(wx)
+
+    def call():
+        stream = torch.cuda.current_stream().cuda_stream
+        rc = lib.frnn_b200_linear_forward(0, wx.data_ptr(), 1, b.data_ptr(), s.data_ptr(), None, out.data_ptr(), last.data_ptr(),
+                                          starts.data_ptr(), exchange.data_ptr(), B, T, N, D, 30, (clean if backward else err).data_ptr(), stream)
+        if rc == 0 and backward:
+            rc = lib.frnn_b200_linear_backward(0, wx.data_ptr(), 1, b.data_ptr(), s.data_ptr(), None, starts.data_ptr(), dh.data_ptr(),
+                                               dl.data_ptr(), d_wx.data_ptr(), db.data_ptr(), d_init.data_ptr(), part.data_ptr(),
+                                               exchange.data_ptr(), B, T, N, D, 30, err.data_ptr(), stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+
+    clean = torch.zeros_like(err)
+    err[4], err[5] = 1, mute
+    call()
+    assert err[0].item() == 106 and clean[0].item() == 0
+    err.zero_()
+    call()
+    assert err[0].item() == 0 and torch.equal(out, want["hidden"]) and torch.equal(last, want["last"])
+    if backward:
+        assert torch.equal(d_wx, want["d_wx"]) and torch.equal(db, want["d_b"]) and torch.equal(d_init, want["d_states"])
+
+
 def test_offsets_past_32_bits(cuda_device):
     """More than 2^32 bytes and 2^31 elements of Wx: the far end of the sequence is that of a call of its own."""
     from flashrnn_b200 import flashrnn_linear
