@@ -140,7 +140,7 @@ class _FusedProjection(torch.autograd.Function):
         ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, z)
         ctx.activation, ctx.shapes, ctx.features = activation, (x.shape, weight.shape), (J, I)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return y[..., :J] if J % 8 else y
+        return y[..., :J].contiguous() if J % 8 else y
 
     @staticmethod
     def backward(ctx, dy):
@@ -196,7 +196,7 @@ def fused_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     ``activation`` is None, ``"relu"``, ``"silu"`` or ``"gelu_tanh"`` (the tanh form of gelu). x, weight and residual are cast to
     bf16 where they are of another type, ``bias`` is bf16 or fp32 (others are cast to fp32). Nothing is rounded before the result.
     Differentiable in all four (once): the gradient at the product, ``dy * activation'(z)``, is rounded to bf16 for the tensor
-    cores; the bias's gradient sums it unrounded. Features that are no multiple of 8 are padded with zeros, at the price of a copy."""
+    cores; the bias's gradient sums it unrounded. Features that are no multiple of 8 are padded with zeros, at the price of copies of operands and result."""
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"Unknown activation {activation}: None, 'relu', 'silu' or 'gelu_tanh'")
     dev, shape = x.device, x.shape
@@ -249,4 +249,4 @@ def _run_product(x, weight, bias, activation, residual, grad: bool):
     if grad:
         return _FusedProjection.apply(x, weight, bias, residual, activation)
     y = _product_forward(*_whole_vectors(x, weight, bias, residual), activation, False)[0]
-    return y[..., :J] if J % 8 else y
+    return y[..., :J].contiguous() if J % 8 else y

@@ -158,6 +158,21 @@ def test_strides_types_and_unwanted_gradients(cuda_device):
     assert torch.equal(xl.grad, step(x, w, None, None, torch.ones_like(dy), None)["x"])
 
 
+@pytest.mark.parametrize("J", [24, 25])
+def test_the_result_is_dense_and_may_be_changed(J, cuda_device):
+    from flashrnn_b200 import fused_projection
+
+    x, w, _, _, dy = make(40, 33, J, 4, cuda_device)
+    leaf = x.clone().requires_grad_(True)
+    y = fused_projection(leaf, w)
+    assert y.is_contiguous() and y.view(5, 8, J).shape == (5, 8, J)
+    y += 1
+    d, = torch.autograd.grad(y, leaf, dy)
+    with torch.no_grad():
+        assert torch.equal(fused_projection(x, w) + 1, y) and fused_projection(x, w).is_contiguous()
+    assert torch.equal(d, step(x, w, None, None, dy, None)["x"])
+
+
 @pytest.mark.parametrize("shape", [(300, 2048, 200), (5000, 128, 2504), (2, 768, 768)], ids=str)
 def test_same_bits_every_time(shape, cuda_device):
     args = make(*shape, 5, cuda_device, bias=torch.float32, residual=True)
