@@ -395,7 +395,11 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       // parked, not polled: sixteen polling warps take issue slots and power from a long sum's tensor cores
       const bool have = __all_sync(0xffffffffu, mbar_wait_bounded<false, false>(smem_u32(&s_acc_full[a]), (li >> 1) & 1, kLimit, abort_flag));
       if (!have) {
-        if (lane == 0) atomicCAS(p.err, 0, kErrWaitMma);
+        if (lane == 0) {
+          atomicCAS(p.err, 0, kErrWaitMma);
+          const uint64_t t0 = global_timer_ns();  // a residual on its way lands before the CTA leaves
+          while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        }
         break;
       }
       tc_fence_after_sync();

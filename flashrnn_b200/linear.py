@@ -36,13 +36,19 @@ def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Option
         last = bias.new_empty((1, B, 1, N, D))
     starts = exchange = err = word = None
     if keep and plan.starts_bytes:
-        starts = bias.new_empty(plan.starts_bytes // 4)
+        # with the exchange buffer behind it: an allocation costs a short call more than 2 % of Wx cost a long one's memory
+        behind = (plan.starts_bytes + 15) // 16 * 16
+        starts = bias.new_empty((behind + plan.exchange_bytes) // 4)
     if plan.exchange_bytes:   # several tiles, which wait for one another
-        exchange = bias.new_empty(plan.exchange_bytes // 4)
+        if starts is None:
+            scratch = bias.new_empty(plan.exchange_bytes // 4)
+            exchange = scratch.data_ptr()
+        else:
+            exchange = starts.data_ptr() + behind
         err, word = _launch_word(dev)
     rc = lib.frnn_b200_linear_forward(
         _lib.LINEAR_CELLS[function], wx.data_ptr(), wx.dtype == torch.bfloat16, bias.data_ptr(), _ptr(initial), _ptr(lengths),
-        hidden.data_ptr(), last.data_ptr(), _ptr(starts), _ptr(exchange), B, T, N, D, 0, err, _stream(dev))
+        hidden.data_ptr(), last.data_ptr(), _ptr(starts), exchange, B, T, N, D, 0, err, _stream(dev))
     if rc:
         _lib.check(rc, "frnn_b200_linear_forward")
     if err is not None:
