@@ -128,6 +128,32 @@ def _launched(holder, what: str) -> None:
         holder.names.append(what)
 
 
+def _gradient_nodes(ctx):
+    """The autograd nodes that a function's gradients go to, and those behind the casts and copies of its arguments (three at most)."""
+    for node, _ in ctx.next_functions:
+        for _ in range(4):
+            if node is None:
+                break
+            yield node
+            behind = node.next_functions
+            node = behind[0][0] if len(behind) == 1 else None
+
+
+def _note_stream(ctx, device: torch.device) -> None:
+    """In an autograd function's forward pass: leaves on the nodes that its gradients go to the stream of the first call that met them.
+    Autograd runs a leaf's node on the stream it was made on and keeps it while any graph of that leaf lives."""
+    stream = _stream(device)
+    for node in _gradient_nodes(ctx):
+        node.metadata.setdefault("frnn_stream", stream)
+
+
+def _refuse_capture(ctx) -> None:
+    """In its backward pass: a capture that autograd would make wait for the default stream, which no capture can, ends the process."""
+    if _capturing() and any(node.metadata.get("frnn_stream") == 0 for node in _gradient_nodes(ctx)):
+        raise RuntimeError("cannot capture this backward pass: an autograd graph of the same inputs, made eagerly on the default stream, "
+                           "is alive; let go of its outputs and losses first, or make it on another stream")
+
+
 _captured_errors: list = []   # error words of launches recorded into CUDA graphs: (err, what), newest last
 
 

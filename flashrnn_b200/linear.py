@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import _dense, _launch_word, _launched, _ptr, _stream, poll_errors
+from .functional import _dense, _launch_word, _launched, _note_stream, _ptr, _refuse_capture, _stream, poll_errors
 
 # function -> gates of Wx and b
 LINEAR_GATES = {"leaky": 2, "lstm": 4}
@@ -59,6 +59,7 @@ def _forward(wx, bias, initial, lengths, function: str, keep: bool, last: Option
 class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, wx, bias, initial, lengths, function: str):
+        _note_stream(ctx, wx.device)
         hidden, last, starts = _forward(wx, bias, initial, lengths, function, True)
         ctx.save_for_backward(wx, bias, initial, lengths, starts)
         ctx.function = function
@@ -79,6 +80,7 @@ class _LinearRecurrence(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, d_hidden, d_last, wx, bias, initial, lengths, starts, dev):
+        _refuse_capture(ctx)
         lib = _lib.load()
         poll_errors()
         B, T, _, N, D = wx.shape

@@ -21,7 +21,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import SIZES, FlashRNNConfig, _dense, _error_word, _launch_word, _launched, _ptr, _stream, _track, flashrnn, poll_errors
+from .functional import (SIZES, FlashRNNConfig, _dense, _error_word, _launch_word, _launched, _note_stream, _ptr, _refuse_capture, _stream,
+                         _track, flashrnn, poll_errors)
 from .linear import _current_device, _refuse_second_derivative
 
 
@@ -133,6 +134,7 @@ def _whole_vectors(x, weight, bias, residual):
 class _FusedProjection(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
+        _note_stream(ctx, x.device)
         need = ctx.needs_input_grad
         J, I = weight.shape
         x, weight, bias, residual = _whole_vectors(x, weight, bias, residual)
@@ -152,6 +154,7 @@ class _FusedProjection(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, dy, dev):
+        _refuse_capture(ctx)
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         if not (need_x or need_w or need_b):
             return None, None, None, dy, None

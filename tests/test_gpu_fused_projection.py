@@ -212,6 +212,32 @@ def test_captured_training_step(cuda_device):
     del graph
 
 
+@pytest.mark.parametrize("dtype", [B16, torch.float32], ids=["bf16", "f32"])
+def test_capture_beside_an_eager_graph(dtype, cuda_device):
+    """Autograd runs a leaf's node on the stream of the oldest graph that lives: the default one, which a capture must not wait for."""
+    from flashrnn_b200 import fused_projection
+
+    torch.manual_seed(20)
+    leaves = [torch.randn(shape, device=cuda_device, dtype=dtype).requires_grad_(True) for shape in ((70, 136), (264, 136), (264,))]
+    call = lambda: fused_projection(*leaves, "silu")  # noqa: E731
+    out, graph = call(), torch.cuda.CUDAGraph()
+    want = torch.autograd.grad(out.float().sum(), leaves, retain_graph=True)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot capture this backward pass"), torch.cuda.graph(graph):
+        torch.autograd.grad(call().float().sum(), leaves)
+    out.float().sum().backward()   # the eager graph is as it was
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    del out, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call().float().sum(), leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    del graph
+
+
 @pytest.mark.parametrize("function", ["leaky", "lstm"])
 def test_a_layer(function, cuda_device):
     """Product into the gates, recurrence, product back into the residual stream: a layer's values and all of its gradients."""

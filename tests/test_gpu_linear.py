@@ -288,6 +288,32 @@ def test_captured_decoding_and_training(cuda_device):
     del graph
 
 
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "bf16"])
+def test_capture_beside_an_eager_graph(dtype, cuda_device):
+    """Autograd runs a leaf's node on the stream of the oldest graph that lives: the default one, which a capture must not wait for."""
+    from flashrnn_b200 import flashrnn_linear
+
+    torch.manual_seed(20)
+    leaves = [torch.randn(shape, device=cuda_device, dtype=dtype).requires_grad_(True) for shape in ((3, 300, 2, 1, 40), (2, 1, 40))]
+    call = lambda: flashrnn_linear(*leaves)[0]  # noqa: E731
+    out, graph = call(), torch.cuda.CUDAGraph()
+    want = torch.autograd.grad(out.float().sum(), leaves, retain_graph=True)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot capture this backward pass"), torch.cuda.graph(graph):
+        torch.autograd.grad(call().float().sum(), leaves)
+    out.float().sum().backward()   # the eager graph is as it was
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    del out, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call().float().sum(), leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    del graph
+
+
 @pytest.mark.parametrize("mute", [0, 1, 7])
 @pytest.mark.parametrize("backward", [False, True], ids=["forward", "backward"])
 def test_a_wait_that_runs_out_is_reported(backward, mute, cuda_device):
