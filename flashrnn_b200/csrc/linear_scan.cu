@@ -25,6 +25,7 @@
 // Walks reach 80 % (leaky, B32 T2048 N32 D128: 309 of 246, 509 of 410).
 #include "../../include/flashrnn_b200.h"
 
+#include "column_sum.cuh"
 #include "frnn_common.cuh"
 
 namespace frnn {
@@ -1003,21 +1004,6 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
   for (int g = 0; g < G; ++g) st_f32_vec<VEC>(p.db_part + (static_cast<size_t>(w.b) * G + g) * p.ND + w.ch, db[g].v);
 }
 
-// out[j] = sum over rows of part[row][j], in a fixed order: 32 columns to a block, its 32 warps take rows in turn.
-__global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict__ part, float* __restrict__ out, long long rows, int cols) {
-  __shared__ float s[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
-  float sum = 0.0f;
-  if (j < cols)
-    for (long long r = warp; r < rows; r += 32) sum += part[r * cols + j];
-  s[warp][lane] = sum;
-  __syncthreads();
-  float v = s[lane][warp];  // column `warp` of this block
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0 && blockIdx.x * 32 + warp < cols) out[blockIdx.x * 32 + warp] = v;
-}
-
 int lin_vec(int ND) { return ND % 4 == 0 ? 4 : 1; }
 int lin_channels(int ND) { return lin_vec(ND) == 1 ? 32 : 64; }
 // Enough channels for every SM to keep its loads in flight without cutting time, or next to no time to cut.
@@ -1157,6 +1143,5 @@ extern "C" int frnn_b200_linear_backward(int function, const void* wx, int wx_bf
   rc = launch(function, wx_bf16, p, true, s);
   if (rc != 0 || rows == 1) return rc;
   const int cols = (function == FRNN_LINEAR_LEAKY ? 2 : 4) * p.ND;
-  linear_db_kernel<<<(cols + 31) / 32, 1024, 0, s>>>(db_part, db, rows, cols);
-  return static_cast<int>(cudaGetLastError());
+  return static_cast<int>(column_sum(db_part, db, rows, cols, s));
 }

@@ -23,6 +23,7 @@
 // without an epilogue 24.7, library 23.2). Start and end of the kernel are 4.6 us.
 #include "../../include/flashrnn_b200.h"
 
+#include "column_sum.cuh"
 #include "frnn_common.cuh"
 
 namespace frnn {
@@ -659,25 +660,6 @@ __global__ void __launch_bounds__(256) product_slope_kernel(const __nv_bfloat16*
   }
 }
 
-// out[j] = sum over rows of part[row][j], in a fixed order.
-__global__ void __launch_bounds__(1024) product_bias_kernel(const float* __restrict__ part, void* __restrict__ out, int out_bf16, int rows, int cols) {
-  __shared__ float s[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
-  float sum = 0.0f;
-  if (j < cols)
-    for (int r = warp; r < rows; r += 32) sum += part[static_cast<long long>(r) * cols + j];
-  s[warp][lane] = sum;
-  __syncthreads();
-  float v = s[lane][warp];
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int col = blockIdx.x * 32 + warp;
-  if (lane == 0 && col < cols) {
-    if (out_bf16) static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(v);
-    else static_cast<float*>(out)[col] = v;
-  }
-}
-
 // How an M x N x K product is cut: columns of a tile; tiles done whole, the rest in parts of K.
 struct Cut { int np, parts, chunks_per_part; long long whole, rest; };
 Cut choose_cut(long long M, long long N, long long K) {
@@ -873,8 +855,8 @@ extern "C" int frnn_b200_product_backward(const void* dy, const void* z, const v
     else product_slope_kernel<FRNN_ACT_NONE><<<grid, 256, 0, s>>>(g, h, d, part, M, outputs);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && dbias != nullptr) {
-      product_bias_kernel<<<(outputs + 31) / 32, 1024, 0, s>>>(db_part, dbias, dbias_bf16, blocks, outputs);
-      e = cudaGetLastError();
+      e = dbias_bf16 ? column_sum(db_part, static_cast<__nv_bfloat16*>(dbias), blocks, outputs, s)
+                     : column_sum(db_part, static_cast<float*>(dbias), blocks, outputs, s);
     }
     if (e != cudaSuccess) return static_cast<int>(e);
   }

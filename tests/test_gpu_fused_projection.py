@@ -105,6 +105,13 @@ def test_values_and_gradients(act, shape, cuda_device):
         assert torch.equal(fused_projection(args[0], args[1], args[2], act, args[3]), got["y"])
 
 
+@pytest.mark.parametrize("bias", [B16, torch.float32], ids=["bf16", "f32"])
+def test_many_parts_of_dbias(bias, cuda_device):
+    """So many rows that their parts of dbias are summed by several CTAs."""
+    args = make(131109, 16, 40, 21, cuda_device, bias=bias)
+    check(step(*args, "silu"), *reference(*args, "silu"))
+
+
 def test_extreme_values(cuda_device):
     """Products past the range of fp16 keep their slopes, NaN and infinities stay in their rows."""
     from flashrnn_b200 import fused_projection

@@ -78,6 +78,20 @@ def test_many_channels(function, dtype, shape, cuda_device):
     L.check(got, ref, L.bounds(ref, wx, b, s, T, dh, dl))
 
 
+# so many rows and tiles that the parts of db are summed by several CTAs
+@pytest.mark.parametrize("shape", [(2500, 2, 1, 30), (80, 3400, 1, 8)], ids=str)
+@pytest.mark.parametrize("function", ["leaky", "lstm"])
+def test_many_parts_of_db(function, shape, cuda_device):
+    from flashrnn_b200 import _lib
+
+    B, T, N, D = shape
+    assert _lib.linear_plan(function, *shape).dbpart_bytes >= 4 * 2048 * L.GATES[function] * N * D
+    wx, b, s, n, dh, dl = make(function, *shape, B16, 21, cuda_device, lengths="ragged")
+    got = step(function, wx, b, s, n, dh, dl)
+    ref = L.run_reference(wx, b, s, function, n, dh, dl)
+    L.check(got, ref, L.bounds(ref, wx, b, s, T, dh, dl))
+
+
 @pytest.mark.parametrize("function", ["leaky", "lstm"])
 @pytest.mark.parametrize("T", [7, 130, 2100])
 def test_padding_is_never_read(function, T, cuda_device):
