@@ -19,8 +19,8 @@
 // has started. Many channels, or next to no time: a thread walks its channels through the whole sequence (below).
 //
 // The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. Tiles reach half of it in bf16 (leaky,
-// B8 T2048 N32 D128: 113 us of 61 forward, 204 of 103 backward) and 75 - 85 % in fp32 (B4 T4096: 144 of 123, 261 of 205): per step and channel 31 instructions (ncu), at
-// 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; two thirds of
+// B8 T2048 N32 D128: 110 us of 61 forward, 205 of 103 backward) and 75 - 85 % in fp32 (B4 T4096: 145 of 123, 250 of 205): per step and
+// channel about 30 instructions (ncu), at 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; two thirds of
 // the instructions are the tile's and not the steps', so smaller tiles lose more (64 steps: 132 us) than their shorter chain gains.
 // Walks reach 80 % (leaky, B32 T2048 N32 D128: 309 of 246, 509 of 410).
 #include "../../include/flashrnn_b200.h"
@@ -539,10 +539,10 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  // The maps of this thread's steps up to each of them. The leaky cell keeps only the last one, and its gates as they came in: making
-  // them again costs less than the room for twice as many warps.
-  constexpr int KEEP = CELL == FRNN_LINEAR_LSTM ? L : 1;
-  V A[KEEP], H[KEEP], a, h;
+  // The LSTM keeps the maps of this thread's steps up to each of them, the leaky cell only the decay of each step: its z's as they came in
+  // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 110 us against 125; with the gates made twice 113).
+  constexpr int MAPS = CELL == FRNN_LINEAR_LSTM ? L : 1, DECAYS = CELL == FRNN_LINEAR_LEAKY ? L : 1;
+  V A[MAPS], H[MAPS], decay[DECAYS], a, h;
   auto gates = [&](int l, V& n, V& v) {
     V x[G];
 #pragma unroll
@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
       h = lin_step(n, v, h);
       a = fma_(n, a, a);
     }
-    if constexpr (KEEP > 1) { A[l] = a; H[l] = h; }
+    if constexpr (MAPS > 1) { A[l] = a; H[l] = h; }
+    else decay[l] = n;
   }
   join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
@@ -575,13 +576,12 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
 #pragma unroll
   for (int l = 0; l < L; ++l) {
     V out;
-    if constexpr (KEEP > 1) {
+    if constexpr (MAPS > 1) {
       out = fma_(A[l], c, H[l]);
       out = sigmoid_times_tanh(scaled<CELL>(raw[l][G - 1], bias[G - 1], G - 1), mul_(out, splat<VEC>(-2.0f * kLog2e)));
     } else {
-      V n, v;
-      gates(l, n, v);
-      out = c = lin_step(n, v, c);
+      const V v = mul_(decay[l], scaled<CELL>(raw[l][1], bias[1], 1));
+      out = c = lin_step(decay[l], v, c);
     }
     if (!at.whole) {
       if (at.t0 + l >= p.T) continue;
