@@ -18,8 +18,8 @@
 // depend on timing, so two calls give the same bits. CTAs take their tiles from a counter, earlier steps first: whoever is waited for
 // has started. Many channels, or next to no time: a thread walks its channels through the whole sequence (below).
 //
-// The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. Tiles reach half of it in bf16 (leaky,
-// B8 T2048 N32 D128: 110 us of 61 forward, 205 of 103 backward) and 75 - 85 % in fp32 (B4 T4096: 145 of 123, 250 of 205): per step and
+// The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. Tiles reach 50 - 60 % of it in bf16 (leaky,
+// B8 T2048 N32 D128: 102 us of 61 forward, 197 of 103 backward) and 83 - 89 % in fp32 (B4 T4096: 138 of 123, 247 of 205): per step and
 // channel about 30 instructions (ncu), at 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; two thirds of
 // the instructions are the tile's and not the steps', so smaller tiles lose more (64 steps: 132 us) than their shorter chain gains.
 // Walks reach 80 % (leaky, B32 T2048 N32 D128: 309 of 246, 509 of 410).
@@ -244,6 +244,8 @@ struct Lanes {
   static constexpr int kSpans = 32 / kRow;               // spans of L steps in a warp
 };
 
+// A tile: place in time, row of channel blocks, b, channel block, the sequence's length.
+struct TileId { int k, row, b, cg, len, mute; };
 // The words that tiles of one (batch row, channel block) exchange: maps [tile][channel] (A, H), states [group][channel].
 struct Exchange {
   uint8_t *maps, *states;
@@ -298,7 +300,18 @@ struct Fetched {
   uint2 map[kTiles][kWords];
   const uint8_t* from;
   int n_channels, count;  // count: tiles of the group in front of this one
-  __device__ __forceinline__ void ask(const LinParams& p, const Exchange& x, int k, int channels) {
+  // Of this thread's channel, what its group starts from: a state, in a row's first group `first` [B][ND] (null: zeros). Asked for here, not
+  // behind the barrier where it is needed: 4 % of a forward pass.
+  uint32_t start;
+  __device__ __forceinline__ void ask(const LinParams& p, const TileId& id, int k, const float* first) {
+    const int c0 = id.cg * CW, channels = min(CW, p.ND - c0);
+    const Exchange x(p, id.row, CW);
+    start = 0u;
+    if (static_cast<int>(threadIdx.x) < channels) {
+      if (k >= kGroup) start = ld_relaxed_gpu_u32(x.states + (static_cast<long long>(k / kGroup) * CW + threadIdx.x) * 4);
+      else if (first != nullptr) start = __float_as_uint(__ldg(first + static_cast<long long>(id.b) * p.ND + c0 + threadIdx.x));
+    }
+    if (p.n_tiles == 1) return;
     from = x.maps + static_cast<long long>(k / kGroup * kGroup) * CW * 8;
     n_channels = channels;
     count = k % kGroup;
@@ -333,32 +346,31 @@ struct Fetched {
 };
 // ... and they are composed in order with the state at the start of the group, which the last tile of the group before hands out.
 template <int CW>
-__device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x, int k, bool mute, int channel, const float2 (*s_prev)[CW], float first,
-                                           float a, float h) {
+__device__ __forceinline__ float lin_carry(const LinParams& p, const Exchange& x, int k, bool mute, int channel, const float2 (*s_prev)[CW],
+                                           uint32_t start, float a, float h) {
   const int group = k / kGroup, at = k % kGroup;
   float ra = 1.0f, rh = 0.0f;
-  for (int q = 0; q < at; ++q) {
+#pragma unroll
+  for (int q = 0; q < kGroup - 1; ++q) {
+    if (q >= at) break;
     const float2 m = s_prev[q][channel];
     rh = fmaf(m.x, rh, m.y);
     ra *= m.x;
   }
-  if (group > 0) {
-    uint32_t v = kXgFill;
+  if (group > 0 && start == kXgFill) {
     lin_poll(p, [&]() {
-      v = ld_relaxed_gpu_u32(x.states + (static_cast<long long>(group) * CW + channel) * 4);
-      return v != kXgFill;
+      start = ld_relaxed_gpu_u32(x.states + (static_cast<long long>(group) * CW + channel) * 4);
+      return start != kXgFill;
     });
-    first = __uint_as_float(v);
   }
-  const float carry = fmaf(ra, first, rh);
+  const float carry = fmaf(ra, __uint_as_float(start), rh);
   if (k + 1 < p.n_tiles && at == kGroup - 1 && !mute)
     st_relaxed_gpu_u32(x.states + (static_cast<long long>(group + 1) * CW + channel) * 4, xg_clean(__float_as_uint(fmaf(a, carry, h))));
   return carry;
 }
 
-// The tile of this CTA, from the counter where tiles wait on one another: k, row, b, channel block, and the row's length. One
-// thread divides for all.
-struct TileId { int k, row, b, cg, len, mute; };
+// The tile of this CTA, from the counter where tiles wait on one another. One thread divides for
+// all (two divisions a thread are 2 % of a tile's time).
 __device__ __forceinline__ TileId lin_tile(const LinParams& p, TileId* shared) {
   if (threadIdx.x == 0) {
     int id = static_cast<int>(blockIdx.x);
@@ -391,14 +403,13 @@ struct Shared {
   float2 prev[kGroup - 1][CW];
 };
 
-// From the maps of the CTA's warps to the value that each of them starts from; warps count backwards in reverse time. `first` [B][ND]
-// (null: zeros) is what the row starts from; done(state, channel, carry, end) is called per channel with its place in [B][ND], what
-// the tile starts from and what it ends with. The maps are in place and a barrier is behind them.
+// From the maps of the CTA's warps to the value that each of them starts from; warps count backwards in reverse time.
+// done(state, channel, carry, end) is called per channel with its place in [B][ND], what the tile starts from and what it ends with. The maps are in place and a barrier is behind them.
 template <int CW, int NW, bool REVERSE, typename F>
-__device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, bool mute, const float* first, Shared<CW, NW>& s, Fetched<CW, NW>& got,
-                                         F done) {
-  const int nw = blockDim.x >> 5, b = row / p.n_cg, c0 = (row % p.n_cg) * CW, n_channels = min(CW, p.ND - c0);
-  const Exchange x(p, row, CW);
+__device__ __forceinline__ void lin_join(const LinParams& p, const TileId& id, int k, Shared<CW, NW>& s, Fetched<CW, NW>& got, F done) {
+  const int nw = blockDim.x >> 5, c0 = id.cg * CW, n_channels = min(CW, p.ND - c0);
+  const bool mute = id.mute != 0;
+  const Exchange x(p, id.row, CW);
   const int c = threadIdx.x;  // a CTA has as many threads as a tile has channels, or more
   float a = 1.0f, h = 0.0f;
   if (c < n_channels) {
@@ -416,9 +427,9 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, boo
     __syncthreads();
   }
   if (c < n_channels) {
-    const long long state = static_cast<long long>(b) * p.ND + c0 + c;
-    float carry = first != nullptr && k < kGroup ? __ldg(first + state) : 0.0f;
-    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, mute, c, s.prev, carry, a, h);
+    const long long state = static_cast<long long>(id.b) * p.ND + c0 + c;
+    float carry = __uint_as_float(got.start);
+    if (p.n_tiles > 1) carry = lin_carry<CW>(p, x, k, mute, c, s.prev, got.start, a, h);
     done(state, c0 + c, carry, fmaf(a, carry, h));
 #pragma unroll 4
     for (int i = 0; i < nw; ++i) {
@@ -433,14 +444,13 @@ __device__ __forceinline__ void lin_join(const LinParams& p, int row, int k, boo
 // This thread's part of a tile.
 template <int VEC, int L, int TILE>
 struct Place {
-  int k, row, b, c0, chl, ch, warp, span, t0, len;
-  bool ok, whole, mute;  // ok: the channels exist; whole: and so do all steps of the warp
+  int k, b, c0, chl, ch, warp, span, t0, len;
+  bool ok, whole;  // ok: the channels exist; whole: and so do all steps of the warp
   __device__ __forceinline__ Place(const LinParams& p, const TileId& id, bool reverse) {
     using W = Lanes<VEC>;
     const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
     k = reverse ? p.n_tiles - 1 - id.k : id.k;
-    row = id.row;
     b = id.b;
     c0 = id.cg * W::kChannels;
     span = lane / W::kRow;
@@ -449,7 +459,6 @@ struct Place {
     t0 = k * TILE + (warp * W::kSpans + span) * L;
     ok = ch < p.ND;
     len = id.len;
-    mute = id.mute != 0;
     whole = k * TILE + (warp + 1) * W::kSpans * L <= len && c0 + W::kChannels <= p.ND;
   }
   __device__ __forceinline__ bool valid(int l) const { return ok && t0 + l < len; }
@@ -535,12 +544,12 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
       }
   }
   Fetched<CW, NW> got;
-  if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), at.k, min(CW, p.ND - at.c0));
+  got.ask(p, s_tile, at.k, p.initial);
   V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
   // The LSTM keeps the maps of this thread's steps up to each of them, the leaky cell only the decay of each step: its z's as they came in
-  // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 110 us against 125; with the gates made twice 113).
+  // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 110 us against 125; with the gates made twice 113; 102 now).
   constexpr int MAPS = CELL == FRNN_LINEAR_LSTM ? L : 1, DECAYS = CELL == FRNN_LINEAR_LEAKY ? L : 1;
   V A[MAPS], H[MAPS], decay[DECAYS], a, h;
   auto gates = [&](int l, V& n, V& v) {
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   }
   join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
-  lin_join<CW, NW, false>(p, at.row, at.k, at.mute, p.initial, s, got, [&](long long state, int channel, float carry, float end) {
+  lin_join<CW, NW, false>(p, s_tile, at.k, s, got, [&](long long state, int channel, float carry, float end) {
     if (p.starts != nullptr && at.k > 0) p.starts[(static_cast<long long>(at.b) * (p.n_tiles - 1) + at.k - 1) * p.ND + channel] = carry;
     if (at.k == p.n_tiles - 1) p.last[state] = end;
   });
@@ -643,7 +652,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     }
   }
   Fetched<CW, NW> got;
-  if (p.n_tiles > 1) got.ask(p, Exchange(p, at.row, CW), kr, min(CW, p.ND - at.c0));
+  got.ask(p, s_tile, kr, p.d_last);
   // the state in front of the tile, channels as in lin_join
   const bool mine = tid < min(CW, p.ND - at.c0);
   float before = 0.0f;
@@ -732,7 +741,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   }
   join_spans<VEC, true>(at.span, A, E, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
-  lin_join<CW, NW, true>(p, at.row, kr, at.mute, p.d_last, s, got, [&](long long state, int, float, float end) {
+  lin_join<CW, NW, true>(p, s_tile, kr, s, got, [&](long long state, int, float, float end) {
     if (at.k == 0 && p.d_initial != nullptr) p.d_initial[state] = end;
   });
   E = fma_(A, at.ok ? load_<VEC>(&s.start[at.warp][at.chl]) : splat<VEC>(0.0f), E);
