@@ -806,12 +806,14 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
 // Many channels: there is no need to cut time. A thread walks its two channels (one, where ND is odd) through the whole sequence, the
 // next steps' loads in flight while it computes; no exchange, a third of the instructions of a tile. The states it keeps for the
 // backward pass are kWalkSteps apart: what the backward walk recomputes between two of them stays in registers.
-// A step takes 80 - 100 ns however many threads there are, until the memory is full, so it depends on the channels B N D who is faster;
-// walk against tile, forward + backward, us: leaky bf16 131072 x T2048 309 + 509, 494 + 813; 65536 220 + 354, 266 + 413; 32768 x T4096 355 +
-// 564, 251 + 419; lstm 131072 773 + 1315, 869 + 1648; 65536 468 + 746, 423 + 802. Channels that are no multiple of four have slower tiles: 48960 x
-// T512 52 + 87, 62 + 114. Up to 16 steps there is nothing to cut: 4 x 1 x 768 2.5 us, 4.9 in a tile.
+// A step takes 80 - 100 ns (LSTM 190 - 230) however many threads there are, until the memory is full, so it depends on the channels B N D who
+// is faster; walk against tile, forward + backward, us, bf16 and fp32: leaky 65536 x T2048 219 + 353, 199 + 382; 81920 250 + 405, 248 + 476;
+// 131072 310 + 522, 396 + 766; fp32 65536 x T1024 163 + 299, 149 + 258; 98304 232 + 381, 227 + 389; 131072 314 + 472, 299 + 514. LSTM 65536 x T1024
+// 232 + 379, 189 + 379; 98304 397 + 584, 281 + 565; 131072 459 + 663, 376 + 746; fp32 98304 420 + 780, 413 + 708; 131072 495 + 922, 574 + 920.
+// Channels that are no multiple of four have slower tiles: 48960 x T512 59 + 96, 70 + 120 (LSTM 102 + 157, 119 + 226). Up to 16 steps there is
+// nothing to cut: 4 x 1 x 768 2.5 us, 4.9 in a tile.
 constexpr int kWalkSteps = 8, kWalkThreads = 64;
-constexpr long long kWalkChannels = 65536, kWalkOddChannels = 32768;
+constexpr long long kWalkChannels = 65536, kWalkLstmChannels = 131072, kWalkOddChannels = 32768;
 
 template <int CELL, int VEC, bool BF16>
 struct Walk {
@@ -1016,7 +1018,10 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
 int lin_vec(int ND) { return ND % 4 == 0 ? 4 : 1; }
 int lin_channels(int ND) { return lin_vec(ND) == 1 ? 32 : 64; }
 // Enough channels for every SM to keep its loads in flight without cutting time, or next to no time to cut.
-bool lin_walk(long long B, int T, long long ND) { return T <= 2 * kWalkSteps || B * ND >= (ND % 4 == 0 ? kWalkChannels : kWalkOddChannels); }
+bool lin_walk(int function, long long B, int T, long long ND) {
+  const long long many = ND % 4 != 0 ? kWalkOddChannels : (function == FRNN_LINEAR_LSTM ? kWalkLstmChannels : kWalkChannels);
+  return T <= 2 * kWalkSteps || B * ND >= many;
+}
 
 template <int CELL, int VEC, bool BF16, bool BACKWARD>
 int launch_walk(const LinParams& p, cudaStream_t s) {
@@ -1047,7 +1052,7 @@ int launch_one(const LinParams& p, bool backward, cudaStream_t s) {
 template <int CELL, bool BF16>
 int launch_vec(const LinParams& p, bool backward, cudaStream_t s) {
   constexpr bool kLstm = CELL == FRNN_LINEAR_LSTM;
-  if (lin_walk(p.B, p.T, p.ND)) {
+  if (lin_walk(CELL, p.B, p.T, p.ND)) {
     constexpr int kBack = kLstm ? 1 : 2;  // two channels of the LSTM's backward walk do not fit the registers
     if (backward) return p.ND % 2 == 0 ? launch_walk<CELL, kBack, BF16, true>(p, s) : launch_walk<CELL, 1, BF16, true>(p, s);
     return p.ND % 2 == 0 ? launch_walk<CELL, 2, BF16, false>(p, s) : launch_walk<CELL, 1, BF16, false>(p, s);
@@ -1094,7 +1099,7 @@ extern "C" int frnn_b200_linear_plan(int function, int B, int T, int N, int D, f
   if (blocks * tiles > 0x7fffffffLL) return -2;
   *out = {};
   out->gates = gates;
-  if (lin_walk(B, T, nd)) {
+  if (lin_walk(function, B, T, nd)) {
     out->tile_steps = kWalkSteps;
     out->tile_channels = nd % 2 == 0 ? 2 : 1;
     out->tiles = 1;

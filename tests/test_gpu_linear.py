@@ -64,7 +64,7 @@ def test_values_and_gradients(function, dtype, shape, cuda_device):
 # so many channels that a thread walks the whole sequence: even and odd widths, lengths around the 8 and 16 steps that it has on
 # their way
 @pytest.mark.parametrize("shape", [(512, 1, 1, 128), (512, 7, 2, 64), (512, 8, 1, 128), (256, 9, 2, 129), (200, 17, 1, 330), (410, 41, 5, 33),
-                                   (1100, 25, 1, 30)], ids=str)
+                                   (1100, 25, 1, 30), (512, 19, 1, 256)], ids=str)
 @pytest.mark.parametrize("dtype", [B16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("function", ["leaky", "lstm"])
 def test_many_channels(function, dtype, shape, cuda_device):
