@@ -20,7 +20,7 @@
 //
 // The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. Tiles reach 50 - 60 % of it in bf16 (leaky,
 // B8 T2048 N32 D128: 102 us of 61 forward, 197 of 103 backward) and 83 - 89 % in fp32 (B4 T4096: 138 of 123, 247 of 205): per step and
-// channel about 30 instructions (ncu), at 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; two thirds of
+// channel 27 instructions (ncu), at 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; more than half of
 // the instructions are the tile's and not the steps', so smaller tiles lose more (64 steps: 132 us) than their shorter chain gains.
 // Walks reach 80 % (leaky, B32 T2048 N32 D128: 309 of 246, 509 of 410).
 #include "../../include/flashrnn_b200.h"
