@@ -226,7 +226,9 @@ def poll_errors(block: bool = False) -> None:
         for device in {err.device for err, _ in _captured_errors}:
             torch.cuda.synchronize(device)
         for err, what in _captured_errors:
-            _raise_device_error(err.tolist(), what + " (in a replayed CUDA graph)")
+            row = err.tolist()
+            if row[0] > 0 and row[0] in _lib.ERROR_TEXT:   # a word of a graph that was never replayed holds whatever was there before
+                _raise_device_error(row, what + " (in a replayed CUDA graph)")
 
 
 class _Recurrence(torch.autograd.Function):

@@ -328,6 +328,28 @@ def test_capture_beside_an_eager_graph(dtype, cuda_device):
     del graph
 
 
+def test_words_of_a_graph_that_was_never_replayed(cuda_device, monkeypatch):
+    """Nothing has zeroed them: what lies there is no error, unless it is a kernel's code."""
+    from flashrnn_b200 import flashrnn_linear, functional, poll_errors
+
+    words = []
+    monkeypatch.setattr(functional, "_captured_errors", words)
+    wx, b, s, _, _, _ = make("leaky", 2, 300, 1, 40, B16, 22, cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        flashrnn_linear(wx, b, s, "leaky")
+    assert len(words) == 1
+    for left_there in (-1, 1065353216):
+        words[0][0].fill_(left_there)
+        poll_errors(block=True)
+    words[0][0][0] = 106
+    with pytest.raises(RuntimeError, match="replayed CUDA graph"):
+        poll_errors(block=True)
+    graph.replay()                     # zeroes it
+    poll_errors(block=True)
+    del graph
+
+
 @pytest.mark.parametrize("mute", [0, 1, 7])
 @pytest.mark.parametrize("backward", [False, True], ids=["forward", "backward"])
 def test_a_wait_that_runs_out_is_reported(backward, mute, cuda_device):
