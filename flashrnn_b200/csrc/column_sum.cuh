@@ -12,6 +12,7 @@ template <typename Out>
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, Out* __restrict__ out, long long rows, int cols) {
   __shared__ float s[32][33], s_part[kColumnSplits][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+  if (gridDim.y > 1) cluster_arrive();  // another CTA's shared memory may be written once that CTA has started
   const long long per = (rows + gridDim.y - 1) / gridDim.y, first = per * blockIdx.y, end = first + per < rows ? first + per : rows;
   float sum = 0.0f;
   if (j < cols) {
@@ -24,6 +25,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (gridDim.y > 1) {  // all of it at the cluster's first CTA
+    cluster_wait();
     if (lane == 0)
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(smem_u32(&s_part[blockIdx.y][warp]), 0)), "f"(v) : "memory");
     cluster_sync_all();
