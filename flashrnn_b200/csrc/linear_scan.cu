@@ -1,10 +1,11 @@
 // Gated linear recurrence: per channel (head, unit) of a batch row
-//   c_t = f_t c_{t-1} + v_t,   f_t = 1 - u_t,   u_t = sigmoid(-(x_f + b_f))
+//   c_t = f_t c_{t-1} + v_t,   f_t = sigmoid(x_f + b_f),   u_t = 1 - f_t
 //   leaky (f, z):       v = u z,                      hidden = c
 //   lstm  (i, f, z, o): v = sigmoid(i) tanh(z),       hidden = sigmoid(o) tanh(c)
 // with x the gate pre-activations Wx[B,T,G,N,D]. There is no recurrent matrix, so a span of steps is the map
-// c -> A c + H with A = prod f, and spans compose: (A2, H2) o (A1, H1) = (A2 A1, A2 H1 + H2). Written with u instead of f the
-// step c + v - u c keeps full precision where f is next to one, which is where errors would add up over the most steps.
+// c -> A c + H with A = prod f, and spans compose: (A2, H2) o (A1, H1) = (A2 A1, A2 H1 + H2). A step is c + (v - u c) where
+// f is 1/2 or more and f c + v where it is less: u keeps its digits where f is next to one, which is where errors would add up over the most
+// steps, f keeps them where it is next to zero, where a large state has to vanish behind a small input.
 //
 // Backward: with dc_t the gradient that reaches c_t through hidden_t, g_t = dc_t + f_{t+1} g_{t+1}; the same scan in reverse
 // time over e_t = f_t (dc_t + e_{t+1}). The gates' gradients need c_{t-1}: it is recomputed from Wx, which has to be read
@@ -211,31 +212,89 @@ __device__ __forceinline__ Vec<N> sigmoid_times_tanh(const Vec<N>& a, const Vec<
   return mul_(fma_(eb, splat<N>(-1.0f), one), rcp_(mul_(da, add_(one, eb))));
 }
 
+// f = sigmoid(x) and u = 1 - f as one number, from log2(e) x: the smaller of the two, f itself or -u, so that neither loses its digits where
+// the other is next to one. With p = 1 where it is -u and 0 where it is f: f = p + m, a step is c -> p c + (m c + v), and f u = |m| - m^2.
+// The least subnormal, added where it would round to zero, keeps its sign; a step that is to leave the state alone has m = 0, v = 0.
+template <int N>
+__device__ __forceinline__ Vec<N> decay_(const Vec<N>& x) {
+  Vec<N> q, m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = exp2_fast(-fabsf(x[i]));
+  m = fma_(q, rcp_(add_(splat<N>(1.0f), q)), splat<N>(__uint_as_float(1u)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) m[i] = __uint_as_float(__float_as_uint(m[i]) | (~__float_as_uint(x[i]) & 0x80000000u));
+  return m;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> side_(const Vec<N>& m) {  // p
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm("set.le.f32.f32 %0, %1, 0f00000000;" : "=f"(r.v[i]) : "f"(m.v[i]));
+  return r;
+}
+// The same, made anew: in a later pass over the steps a register to hold it costs more than the instruction.
+template <int N>
+__device__ __forceinline__ Vec<N> side_again(const Vec<N>& m) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("set.le.f32.f32 %0, %1, 0f00000000;" : "=f"(r.v[i]) : "f"(m.v[i]));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> pick_(const Vec<N>& m, const Vec<N>& open, const Vec<N>& shut) {  // by p
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = m[i] <= 0.0f ? open[i] : shut[i];
+  return r;
+}
+template <int N>
+__device__ __forceinline__ Vec<N> minus_(const Vec<N>& a, const Vec<N>& b) { return fma_(b, splat<N>(-1.0f), a); }
+template <int N>
+__device__ __forceinline__ Vec<N> minus_u(const Vec<N>& m, const Vec<N>& p) { return add_(m, add_(p, splat<N>(-1.0f))); }
+template <int N>
+__device__ __forceinline__ Vec<N> minus_fu(const Vec<N>& m) {
+  Vec<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = -fabsf(m[i]);
+  return fma_(m, m, r);
+}
+// f x with one rounding; where p is at hand for other things too, and where it is not.
+template <int N>
+__device__ __forceinline__ Vec<N> times_f(const Vec<N>& m, const Vec<N>& p, const Vec<N>& x) { return fma_(m, x, mul_(p, x)); }
+template <int N>
+__device__ __forceinline__ Vec<N> times_f(const Vec<N>& m, const Vec<N>& x) { return fma_(m, x, pick_(m, x, splat<N>(0.0f))); }
+
 // Gates arrive as scale(g) (Wx + b): the factor that the exponentials want goes into one fused multiply-add with the bias. What a
-// step does is kept as n = -u and v: c + v - u c = fma(n, c, c + v).
+// step does is kept as m and w; `step` takes a state through it, `first` the state zero. The leaky cell's w is z: with d = c - z its step
+// is c - u d or z + f d, c + m d or z + m d. The LSTM's is v.
 // kTile: steps of a tile. The LSTM's backward pass holds five values per step and channel: 64 steps leave room for two CTAs.
 template <int CELL> struct LinCell;
 template <> struct LinCell<FRNN_LINEAR_LEAKY> {
   static constexpr int G = 2, kTile = 128;
-  static __device__ __forceinline__ constexpr float scale(int g) { return g == 0 ? kLog2e : -1.0f; }  // the second gate is -z
+  static __device__ __forceinline__ constexpr float scale(int g) { return g == 0 ? kLog2e : 1.0f; }
   template <int N>
-  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& n, Vec<N>& v) {
-    n = rcp_(fma_(exp2_(x[0]), splat<N>(-1.0f), splat<N>(-1.0f)));
-    v = mul_(n, x[1]);
+  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& m, Vec<N>& w) {
+    m = decay_(x[0]);
+    w = x[1];
   }
+  template <int N>
+  static __device__ __forceinline__ Vec<N> step(const Vec<N>& m, const Vec<N>& w, const Vec<N>& c) { return fma_(m, minus_(c, w), pick_(m, c, w)); }
+  template <int N>
+  static __device__ __forceinline__ Vec<N> first(const Vec<N>& m, const Vec<N>& w) { return step(m, w, splat<N>(0.0f)); }
 };
 template <> struct LinCell<FRNN_LINEAR_LSTM> {
   static constexpr int G = 4, kTile = 64;
   static __device__ __forceinline__ constexpr float scale(int g) { return g == 1 ? kLog2e : (g == 2 ? -2.0f * kLog2e : -kLog2e); }
   template <int N>
-  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& n, Vec<N>& v) {
-    n = rcp_(fma_(exp2_(x[1]), splat<N>(-1.0f), splat<N>(-1.0f)));
-    v = sigmoid_times_tanh(x[0], x[2]);
+  static __device__ __forceinline__ void gates(const Vec<N>* x, Vec<N>& m, Vec<N>& w) {
+    m = decay_(x[1]);
+    w = sigmoid_times_tanh(x[0], x[2]);
   }
+  template <int N>
+  static __device__ __forceinline__ Vec<N> step(const Vec<N>& m, const Vec<N>& w, const Vec<N>& c) { return fma_(side_(m), c, fma_(m, c, w)); }
+  template <int N>
+  static __device__ __forceinline__ Vec<N> first(const Vec<N>&, const Vec<N>& w) { return w; }
 };
-
-template <int N>
-__device__ __forceinline__ Vec<N> lin_step(const Vec<N>& n, const Vec<N>& v, const Vec<N>& c) { return fma_(n, c, add_(c, v)); }
 
 template <int VEC>
 struct Lanes {
@@ -552,26 +611,26 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 110 us against 125; with the gates made twice 113; 102 now).
   constexpr int MAPS = CELL == FRNN_LINEAR_LSTM ? L : 1, DECAYS = CELL == FRNN_LINEAR_LEAKY ? L : 1;
   V A[MAPS], H[MAPS], decay[DECAYS], a, h;
-  auto gates = [&](int l, V& n, V& v) {
+  auto gates = [&](int l, V& m, V& w) {
     V x[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
-    Cell::gates(x, n, v);
-    if (!at.whole && !at.valid(l)) n = v = splat<VEC>(0.0f);  // a step behind the end of a sequence leaves its state alone
+    Cell::gates(x, m, w);
+    if (!at.whole && !at.valid(l)) m = w = splat<VEC>(0.0f);  // a step behind the end of a sequence leaves its state alone
   };
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    V n, v;
-    gates(l, n, v);
+    V m, w;
+    gates(l, m, w);
     if (l == 0) {
-      a = add_(splat<VEC>(1.0f), n);
-      h = v;
+      a = times_f(m, splat<VEC>(1.0f));
+      h = Cell::first(m, w);
     } else {
-      h = lin_step(n, v, h);
-      a = fma_(n, a, a);
+      h = Cell::step(m, w, h);
+      a = times_f(m, a);
     }
     if constexpr (MAPS > 1) { A[l] = a; H[l] = h; }
-    else decay[l] = n;
+    else decay[l] = m;
   }
   join_spans<VEC, false>(at.span, a, h, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
@@ -589,8 +648,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
       out = fma_(A[l], c, H[l]);
       out = sigmoid_times_tanh(scaled<CELL>(raw[l][G - 1], bias[G - 1], G - 1), mul_(out, splat<VEC>(-2.0f * kLog2e)));
     } else {
-      const V v = mul_(decay[l], scaled<CELL>(raw[l][1], bias[1], 1));
-      out = c = lin_step(decay[l], v, c);
+      out = c = Cell::step(decay[l], scaled<CELL>(raw[l][1], bias[1], 1), c);
     }
     if (!at.whole) {
       if (at.t0 + l >= p.T) continue;
@@ -663,31 +721,31 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  // n = -u; the state in front of each step; the LSTM's i and z
-  V n[L], prev[L], si[LSTM ? L : 1], tz[LSTM ? L : 1];
+  // the decays; the state in front of each step (leaky: less its z); the LSTM's i and z
+  V m[L], prev[L], si[LSTM ? L : 1], tz[LSTM ? L : 1];
 #pragma unroll
   for (int l = 0; l < L; ++l) {
     V x[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
     if constexpr (LSTM) {
-      n[l] = rcp_(fma_(exp2_(x[1]), splat<VEC>(-1.0f), splat<VEC>(-1.0f)));
+      m[l] = decay_(x[1]);
       sigmoid_tanh(x[0], x[2], si[l], tz[l]);
       prev[l] = mul_(si[l], tz[l]);
     } else {
-      Cell::gates(x, n[l], prev[l]);  // v, until the states are known
+      Cell::gates(x, m[l], prev[l]);  // w, until the states are known
     }
   }
   if (!at.whole) {
 #pragma unroll
     for (int l = 0; l < L; ++l)
-      if (!at.valid(l)) n[l] = prev[l] = splat<VEC>(0.0f);
+      if (!at.valid(l)) m[l] = prev[l] = splat<VEC>(0.0f);
   }
-  V A = add_(splat<VEC>(1.0f), n[0]), H = prev[0];
+  V A = add_(side_(m[0]), m[0]), H = Cell::first(m[0], prev[0]);
 #pragma unroll
   for (int l = 1; l < L; ++l) {
-    H = lin_step(n[l], prev[l], H);
-    A = fma_(n[l], A, A);
+    H = Cell::step(m[l], prev[l], H);
+    A = times_f(m[l], side_(m[l]), A);
   }
   join_spans<VEC, false>(at.span, A, H, &f_a[at.warp][at.chl], &f_h[at.warp][at.chl]);
   __syncthreads();
@@ -711,9 +769,9 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   };
 #pragma unroll
   for (int l = 0; l < L; ++l) {
-    const V v = prev[l];
-    prev[l] = c;
-    c = lin_step(n[l], v, c);
+    const V w = prev[l];
+    prev[l] = LSTM ? c : minus_(c, w);
+    c = Cell::step(m[l], w, c);
     if constexpr (LSTM) {
       V o, tc;
       sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c, splat<VEC>(-2.0f * kLog2e)), o, tc);
@@ -730,14 +788,13 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     }
   }
   // what leaves this thread's steps towards earlier ones
-  V E = d_state(L - 1);
-  E = fma_(n[L - 1], E, E);
-  A = add_(splat<VEC>(1.0f), n[L - 1]);
+  A = add_(side_again(m[L - 1]), m[L - 1]);
+  V E = mul_(A, d_state(L - 1));
 #pragma unroll
   for (int l = L - 2; l >= 0; --l) {
-    const V g = add_(d_state(l), E);
-    E = fma_(n[l], g, g);
-    A = fma_(n[l], A, A);
+    const V g = add_(d_state(l), E), side = side_again(m[l]);
+    E = times_f(m[l], side, g);
+    A = times_f(m[l], side, A);
   }
   join_spans<VEC, true>(at.span, A, E, &s.a[at.warp][at.chl], &s.h[at.warp][at.chl]);
   __syncthreads();
@@ -750,18 +807,17 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   for (int l = L - 1; l >= 0; --l) {
     constexpr int kHere = LSTM ? 3 : G;  // gates whose gradients are stored here
     V d[kHere];
-    const V g = add_(d_state(l), E), minus = splat<VEC>(-1.0f);
-    const V q = fma_(n[l], n[l], n[l]);  // -u (1 - u)
-    E = fma_(n[l], g, g);
+    const V g = add_(d_state(l), E), minus = splat<VEC>(-1.0f), side = side_again(m[l]), q = minus_fu(m[l]);
+    E = times_f(m[l], side, g);
     if constexpr (LSTM) {
       const V gi = mul_(g, si[l]), one = splat<VEC>(1.0f);
       d[0] = mul_(mul_(gi, tz[l]), fma_(si[l], minus, one));
       d[1] = mul_(mul_(g, prev[l]), mul_(q, minus));
       d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
     } else {
-      const V mz = scaled<CELL>(raw[l][1], bias[1], 1), mg = mul_(g, minus);  // -z, -g
-      d[0] = mul_(mul_(mg, q), add_(prev[l], mz));
-      d[1] = mul_(mg, n[l]);
+      const V mg = mul_(g, minus);
+      d[0] = mul_(mul_(mg, q), prev[l]);
+      d[1] = mul_(mg, minus_u(m[l], side));
     }
     if (!at.whole && !at.valid(l)) {
 #pragma unroll
@@ -868,18 +924,14 @@ __global__ void __launch_bounds__(kWalkThreads, CELL == FRNN_LINEAR_LSTM ? 1 : 7
   auto steps = [&](const Pack<VEC, BF16> (&raw)[S][G], int t) {
     if (t > 0 && p.starts != nullptr) st_f32_vec<VEC>(p.starts + (static_cast<size_t>(w.b) * last_kept + t / S - 1) * p.ND + w.ch, c.v);
     uint8_t* to = static_cast<uint8_t*>(p.hidden) + (static_cast<size_t>(w.b) * p.T + t) * w.gate + static_cast<size_t>(w.ch) * (BF16 ? 2 : 4);
-    V n[S], v[S];
 #pragma unroll
     for (int l = 0; l < S; ++l) {
-      V x[G];
+      V x[G], m, in;
 #pragma unroll
       for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
-      Cell::gates(x, n[l], v[l]);
-    }
-#pragma unroll
-    for (int l = 0; l < S; ++l) {
+      Cell::gates(x, m, in);
       if (t + l < w.len) {
-        c = lin_step(n[l], v[l], c);
+        c = Cell::step(m, in, c);
         V out = c;
         if constexpr (CELL == FRNN_LINEAR_LSTM)
           out = sigmoid_times_tanh(scaled<CELL>(raw[l][G - 1], bias[G - 1], G - 1), mul_(c, splat<VEC>(-2.0f * kLog2e)));
@@ -938,29 +990,29 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
   V E = p.d_last != nullptr ? load_<VEC>(p.d_last + state) : splat<VEC>(0.0f);
   const V minus = splat<VEC>(-1.0f), one = splat<VEC>(1.0f);
   auto steps = [&](const Pack<VEC, BF16> (&raw)[S][G], const Pack<VEC, BF16> (&dh)[S][1], V c, int t) {
-    V n[S], prev[S], si[LSTM ? S : 1], tz[LSTM ? S : 1], sum[G];
+    V m[S], prev[S], si[LSTM ? S : 1], tz[LSTM ? S : 1], sum[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) sum[g] = splat<VEC>(0.0f);
 #pragma unroll
     for (int l = 0; l < S; ++l) {
-      V x[G], v;
+      V x[G], in;
 #pragma unroll
       for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
       if constexpr (LSTM) {
-        n[l] = rcp_(fma_(exp2_(x[1]), minus, minus));
+        m[l] = decay_(x[1]);
         sigmoid_tanh(x[0], x[2], si[l], tz[l]);
-        v = mul_(si[l], tz[l]);
+        in = mul_(si[l], tz[l]);
       } else {
-        Cell::gates(x, n[l], v);
+        Cell::gates(x, m[l], in);
       }
-      prev[l] = c;
-      c = lin_step(n[l], v, c);
+      prev[l] = LSTM ? c : minus_(c, in);
+      c = Cell::step(m[l], in, c);
     }
 #pragma unroll
     for (int l = S - 1; l >= 0; --l) {
       if (t + l < w.len) {
         V d[G], g = dh[l][0].get();
-        const V q = fma_(n[l], n[l], n[l]);  // -u (1 - u)
+        const V side = side_again(m[l]), q = minus_fu(m[l]);
         if constexpr (LSTM) {
           V o, tc;
           const V c_l = l == S - 1 ? c : prev[l == S - 1 ? l : l + 1];
@@ -974,11 +1026,11 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
           d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
         } else {
           g = add_(g, E);
-          const V mz = scaled<CELL>(raw[l][1], bias[1], 1), mg = mul_(g, minus);  // -z, -g
-          d[0] = mul_(mul_(mg, q), add_(prev[l], mz));
-          d[1] = mul_(mg, n[l]);
+          const V mg = mul_(g, minus);
+          d[0] = mul_(mul_(mg, q), prev[l]);
+          d[1] = mul_(mg, minus_u(m[l], side));
         }
-        E = fma_(n[l], g, g);
+        E = times_f(m[l], side, g);
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           sum[j] = add_(sum[j], d[j]);

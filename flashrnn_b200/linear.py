@@ -130,7 +130,9 @@ def flashrnn_linear(Wx: torch.Tensor, b: torch.Tensor, states: Optional[torch.Te
     behind a row's length leave its state alone, so ``last`` is the state at its end, and their hidden states and gradients are
     zeros, whatever Wx holds there.
 
-    A state that becomes infinite turns into a NaN one step later, in its channel only (its decay is infinity minus infinity).
+    A state that becomes infinite may turn into a NaN later, in its channel only: a decay of 1/2 or more takes a part of it away, infinity
+    from infinity, and over many steps it is multiplied by a decay that has become zero. Sums of a state and its input beyond the range of
+    fp32 count as infinite.
 
     ``last_out`` (without gradients only) is written and returned as ``last``; it may be ``states`` itself, which a captured
     decoding step then updates in place.
