@@ -198,18 +198,39 @@ struct Pack {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-// sigmoid(x) and tanh(y) from a = -log2(e) x and b = -2 log2(e) y with one reciprocal for both: 1 / (1 + 2^a) and
-// (1 - 2^b) / (1 + 2^b). The bounds keep the product of the denominators in range; past them the results are 0 and -1 anyway.
+// tanh(y) as num / den, from b = -2 log2(e) y: with e = 2^-|b| it is (1 - e) / (1 + e) with the sign of y. That difference loses the digits of
+// a small y: below 1/8 it is y - y^3/3 + 2 y^5/15, the start of tanh's series; what is left out of it is 2^-22 of y.
 template <int N>
-__device__ __forceinline__ void sigmoid_tanh(const Vec<N>& a, const Vec<N>& b, Vec<N>& s, Vec<N>& t) {
-  const Vec<N> one = splat<N>(1.0f), eb = exp2_(min_(b, 43.0f)), da = add_(one, exp2_(min_(a, 80.0f))), db = add_(one, eb), r = rcp_(mul_(da, db));
-  s = mul_(db, r);
-  t = mul_(fma_(eb, splat<N>(-1.0f), one), mul_(da, r));
+__device__ __forceinline__ void tanh_(const Vec<N>& b, Vec<N>& e, Vec<N>& num, Vec<N>& den) {
+  constexpr float k = 0.34657359027997264f, kSmall = 0.125f / k;  // y = -k b
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = exp2_fast(-fabsf(b[i]));
+  const Vec<N> one = splat<N>(1.0f), w = mul_(b, b), far = fma_(e, splat<N>(-1.0f), one);
+  den = add_(one, e);
+  Vec<N> near = fma_(w, splat<N>(-k * k * k * k * k * 2.0f / 15.0f), splat<N>(k * k * k / 3.0f));
+  near = mul_(mul_(fma_(w, near, splat<N>(-k)), b), den);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    num[i] = fabsf(b[i]) < kSmall ? near[i] : __uint_as_float(__float_as_uint(far[i]) | (~__float_as_uint(b[i]) & 0x80000000u));
+}
+// sigmoid(x) and tanh(y) from a = -log2(e) x and b = -2 log2(e) y with one reciprocal for both, and what their slopes take, 1 - sigmoid(x) and
+// 1 - tanh(y)^2 = 4 e / (1 + e)^2, not by subtraction, which would lose the digits of a saturated gate's. The bound keeps the
+// product of the denominators in range; past it the sigmoid is 2^-120.
+template <int N>
+__device__ __forceinline__ void sigmoid_tanh(const Vec<N>& a, const Vec<N>& b, Vec<N>& s, Vec<N>& rest, Vec<N>& t, Vec<N>& slope) {
+  Vec<N> e, num, den;
+  tanh_(b, e, num, den);
+  const Vec<N> ea = exp2_(min_(a, 120.0f)), da = add_(splat<N>(1.0f), ea), r = rcp_(mul_(da, den)), inv = mul_(da, r);
+  s = mul_(den, r);
+  rest = mul_(ea, s);
+  t = mul_(num, inv);
+  slope = mul_(mul_(e, splat<N>(4.0f)), mul_(inv, inv));
 }
 template <int N>
 __device__ __forceinline__ Vec<N> sigmoid_times_tanh(const Vec<N>& a, const Vec<N>& b) {
-  const Vec<N> one = splat<N>(1.0f), eb = exp2_(min_(b, 43.0f)), da = add_(one, exp2_(min_(a, 80.0f)));
-  return mul_(fma_(eb, splat<N>(-1.0f), one), rcp_(mul_(da, add_(one, eb))));
+  Vec<N> e, num, den;
+  tanh_(b, e, num, den);
+  return mul_(num, rcp_(mul_(add_(splat<N>(1.0f), exp2_(min_(a, 120.0f))), den)));
 }
 
 // f = sigmoid(x) and u = 1 - f as one number, from log2(e) x: the smaller of the two, f itself or -u, so that neither loses its digits where
@@ -721,8 +742,8 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
   V bias[G];
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
-  // the decays; the state in front of each step (leaky: less its z); the LSTM's i and z
-  V m[L], prev[L], si[LSTM ? L : 1], tz[LSTM ? L : 1];
+  // the decays; the state in front of each step (leaky: less its z); the slopes of the LSTM's v by i and z
+  V m[L], prev[L], by_i[LSTM ? L : 1], by_z[LSTM ? L : 1];
 #pragma unroll
   for (int l = 0; l < L; ++l) {
     V x[G];
@@ -730,8 +751,11 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
     if constexpr (LSTM) {
       m[l] = decay_(x[1]);
-      sigmoid_tanh(x[0], x[2], si[l], tz[l]);
-      prev[l] = mul_(si[l], tz[l]);
+      V i, rest, z, slope;
+      sigmoid_tanh(x[0], x[2], i, rest, z, slope);
+      prev[l] = mul_(i, z);
+      by_i[l] = mul_(prev[l], rest);
+      by_z[l] = mul_(i, slope);
     } else {
       Cell::gates(x, m[l], prev[l]);  // w, until the states are known
     }
@@ -773,11 +797,11 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     prev[l] = LSTM ? c : minus_(c, w);
     c = Cell::step(m[l], w, c);
     if constexpr (LSTM) {
-      V o, tc;
-      sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c, splat<VEC>(-2.0f * kLog2e)), o, tc);
-      const V dh_o = mul_(raw_dh[l].get(), o), minus = splat<VEC>(-1.0f), one = splat<VEC>(1.0f);
-      dc[l] = mul_(dh_o, fma_(mul_(tc, minus), tc, one));
-      V d_o = mul_(mul_(dh_o, tc), fma_(o, minus, one));
+      V o, rest, tc, slope;
+      sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c, splat<VEC>(-2.0f * kLog2e)), o, rest, tc, slope);
+      const V dh_o = mul_(raw_dh[l].get(), o);
+      dc[l] = mul_(dh_o, slope);
+      V d_o = mul_(mul_(dh_o, tc), rest);
       if (!at.whole && !at.valid(l)) dc[l] = d_o = splat<VEC>(0.0f);
       db[3] = add_(db[3], d_o);
       if (at.whole || (at.ok && at.t0 + l < p.T)) {
@@ -810,10 +834,9 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
     const V g = add_(d_state(l), E), minus = splat<VEC>(-1.0f), side = side_again(m[l]), q = minus_fu(m[l]);
     E = times_f(m[l], side, g);
     if constexpr (LSTM) {
-      const V gi = mul_(g, si[l]), one = splat<VEC>(1.0f);
-      d[0] = mul_(mul_(gi, tz[l]), fma_(si[l], minus, one));
+      d[0] = mul_(g, by_i[l]);
       d[1] = mul_(mul_(g, prev[l]), mul_(q, minus));
-      d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
+      d[2] = mul_(g, by_z[l]);
     } else {
       const V mg = mul_(g, minus);
       d[0] = mul_(mul_(mg, q), prev[l]);
@@ -909,7 +932,7 @@ struct Walk {
 };
 
 template <int CELL, int VEC, bool BF16>
-__global__ void __launch_bounds__(kWalkThreads, CELL == FRNN_LINEAR_LSTM ? 1 : 7) linear_fwd_walk_kernel(const LinParams p) {
+__global__ void __launch_bounds__(kWalkThreads, CELL != FRNN_LINEAR_LSTM ? 7 : VEC == 1 ? 6 : 1) linear_fwd_walk_kernel(const LinParams p) {
   using W = Walk<CELL, VEC, BF16>;
   using Cell = LinCell<CELL>;
   using V = Vec<VEC>;
@@ -988,9 +1011,9 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
     return p.initial != nullptr ? load_<VEC>(p.initial + state) : splat<VEC>(0.0f);
   };
   V E = p.d_last != nullptr ? load_<VEC>(p.d_last + state) : splat<VEC>(0.0f);
-  const V minus = splat<VEC>(-1.0f), one = splat<VEC>(1.0f);
+  const V minus = splat<VEC>(-1.0f);
   auto steps = [&](const Pack<VEC, BF16> (&raw)[S][G], const Pack<VEC, BF16> (&dh)[S][1], V c, int t) {
-    V m[S], prev[S], si[LSTM ? S : 1], tz[LSTM ? S : 1], sum[G];
+    V m[S], prev[S], by_i[LSTM ? S : 1], by_z[LSTM ? S : 1], sum[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) sum[g] = splat<VEC>(0.0f);
 #pragma unroll
@@ -1000,8 +1023,11 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
       for (int g = 0; g < G; ++g) x[g] = scaled<CELL>(raw[l][g], bias[g], g);
       if constexpr (LSTM) {
         m[l] = decay_(x[1]);
-        sigmoid_tanh(x[0], x[2], si[l], tz[l]);
-        in = mul_(si[l], tz[l]);
+        V i, rest, z, slope;
+        sigmoid_tanh(x[0], x[2], i, rest, z, slope);
+        in = mul_(i, z);
+        by_i[l] = mul_(in, rest);
+        by_z[l] = mul_(i, slope);
       } else {
         Cell::gates(x, m[l], in);
       }
@@ -1014,16 +1040,15 @@ __global__ void __launch_bounds__(kWalkThreads, 7) linear_bwd_walk_kernel(const 
         V d[G], g = dh[l][0].get();
         const V side = side_again(m[l]), q = minus_fu(m[l]);
         if constexpr (LSTM) {
-          V o, tc;
+          V o, rest, tc, slope;
           const V c_l = l == S - 1 ? c : prev[l == S - 1 ? l : l + 1];
-          sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c_l, splat<VEC>(-2.0f * kLog2e)), o, tc);
+          sigmoid_tanh(scaled<CELL>(raw[l][3], bias[3], 3), mul_(c_l, splat<VEC>(-2.0f * kLog2e)), o, rest, tc, slope);
           const V dh_o = mul_(g, o);
-          d[3] = mul_(mul_(dh_o, tc), fma_(o, minus, one));
-          g = fma_(dh_o, fma_(mul_(tc, minus), tc, one), E);
-          const V gi = mul_(g, si[l]);
-          d[0] = mul_(mul_(gi, tz[l]), fma_(si[l], minus, one));
+          d[3] = mul_(mul_(dh_o, tc), rest);
+          g = fma_(dh_o, slope, E);
+          d[0] = mul_(g, by_i[l]);
           d[1] = mul_(mul_(g, prev[l]), mul_(q, minus));
-          d[2] = mul_(gi, fma_(mul_(tz[l], minus), tz[l], one));
+          d[2] = mul_(g, by_z[l]);
         } else {
           g = add_(g, E);
           const V mg = mul_(g, minus);

@@ -1,5 +1,5 @@
 """flashrnn_linear element by element within the bounds of tests/_linear_error.py: states that are large against what comes in, forget
-gates that are nearly shut."""
+gates that are nearly shut, inputs near zero, gates at the ends of their functions."""
 
 import pytest
 import torch
@@ -29,7 +29,7 @@ def case(function, kind, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("kind", ["plain", "resets"])
+@pytest.mark.parametrize("kind", ["plain", "resets", "small"])
 @pytest.mark.parametrize("shape", LEAKY)
 def test_leaky(shape, kind, dtype, cuda_device):
     args = case("leaky", kind, shape, dtype)
@@ -47,3 +47,11 @@ def test_forget_gate_of_the_lstm(shape, dtype, cuda_device):
     got["d_wx"] = got["d_wx"][:, :, 1]
     ref["d_wx"] = tuple(t[:, :, 1] for t in ref["d_wx"])
     E.check(got, ref, ["last", "d_states", "d_wx"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["plain", "resets", "small", "saturated"])
+@pytest.mark.parametrize("shape", LSTM)
+def test_lstm(shape, kind, dtype, cuda_device):
+    args = case("lstm", kind, shape, dtype)
+    E.check(run("lstm", *args, cuda_device, dtype), E.evaluate(*args[:3], "lstm", *args[3:]))
