@@ -201,9 +201,9 @@ def poll_errors(block: bool = False) -> None:
             return
         _last_poll = now
     with _blocks_lock:
-        for key, block in list(_blocks.items()):
-            block.close()
-            if block.closed == block.given:       # nothing on the way: blocks of finished threads and old streams go
+        for key, words in list(_blocks.items()):
+            words.close()
+            if words.closed == words.given:       # nothing on the way: blocks of finished threads and old streams go
                 del _blocks[key]
     keep = []
     try:
