@@ -380,7 +380,8 @@ struct Fetched {
   uint2 map[kTiles][kWords];
   const uint8_t* from;
   int n_channels, count;  // count: tiles of the group in front of this one
-  // Of this thread's channel, what its group starts from: a state, in a row's first group `first` [B][ND] (null: zeros). Asked for here, not
+  // Of this thread's channel, what its group starts from: a state, in a row's first group `first` [B][ND] (null: zeros; an ordinary load: with one
+  // tile the same thread may write its last state there). Asked for here, not
   // behind the barrier where it is needed: 4 % of a forward pass.
   uint32_t start;
   __device__ __forceinline__ void ask(const LinParams& p, const TileId& id, int k, const float* first) {
@@ -389,7 +390,7 @@ struct Fetched {
     start = 0u;
     if (static_cast<int>(threadIdx.x) < channels) {
       if (k >= kGroup) start = ld_relaxed_gpu_u32(x.states + (static_cast<long long>(k / kGroup) * CW + threadIdx.x) * 4);
-      else if (first != nullptr) start = __float_as_uint(__ldg(first + static_cast<long long>(id.b) * p.ND + c0 + threadIdx.x));
+      else if (first != nullptr) start = __float_as_uint(first[static_cast<long long>(id.b) * p.ND + c0 + threadIdx.x]);
     }
     if (p.n_tiles == 1) return;
     from = x.maps + static_cast<long long>(k / kGroup * kGroup) * CW * 8;
