@@ -135,7 +135,7 @@ def flashrnn_linear(Wx: torch.Tensor, b: torch.Tensor, states: Optional[torch.Te
     fp32 count as infinite.
 
     ``last_out`` (without gradients only) is written and returned as ``last``; it may be ``states`` itself, which a captured
-    decoding step then updates in place.
+    decoding step then updates in place. Where it shares memory with another input, that is written once the call has read it.
     """
     if function not in LINEAR_GATES:
         raise ValueError(f"Unknown function {function}: flashrnn_linear has {', '.join(LINEAR_GATES)}")
@@ -192,15 +192,23 @@ def _run(wx, b, states, function, lengths, last_out, grad):
     out = last_out
     if out is not None and out.data_ptr() % 16:
         out = None
-    if out is not None and states is not None and states.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
-        # a call of several steps may read `states` after other parts of `last` are written, and a step may where the two overlap
-        # without being the same: a buffer in between
-        if wx.shape[1] > 1 or states.data_ptr() != out.data_ptr():
+    if out is not None:
+        # a call of several steps may read `states` after other parts of `last` are written, and so may a step where the two overlap without
+        # being the same, or where `last_out` lies over another input: a buffer in between
+        if _overlap(wx, out) or _overlap(b, out) or (lengths is not None and _overlap(lengths, out)):
+            out = None
+        elif states is not None and _overlap(states, out) and (wx.shape[1] > 1 or states.data_ptr() != out.data_ptr()):
             out = None
     hidden, last, _ = _forward(wx, b, states, lengths, function, False, out)
     if last_out is not None and out is None:
         last = last_out.copy_(last)
     return hidden, last
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    first, second = a.data_ptr(), b.data_ptr()
+    return first < second + b.nbytes and second < first + a.nbytes
 
 
 def _state(t: torch.Tensor) -> torch.Tensor:
