@@ -788,8 +788,8 @@ int rows_launch(const ProductParams& p, const void* x, const void* w, const void
 
 bool bad_sizes(int64_t rows, int outputs, int inputs) { return rows < 1 || outputs < 1 || inputs < 1; }
 bool unsupported(int64_t rows, int outputs, int inputs) {
-  // coordinates and tile counts are 32-bit; 16-byte rows
-  return rows > 0x7fffff00LL || outputs > 0x7fffff00 || inputs > 0x7fffff00 || outputs % 8 != 0 || inputs % 8 != 0 ||
+  // coordinates and tile counts are 32-bit, and the k's of product_rows_kernel are counted past the end by up to 511; 16-byte rows
+  return rows > 0x7fffff00LL || outputs > 0x7fffff00 || inputs > 0x7ffffe00 || outputs % 8 != 0 || inputs % 8 != 0 ||
          rows * outputs / 8 > 0x7fffffffLL * 256 || static_cast<long long>(inputs) * outputs / 8 > 0x7fffffffLL * 256;
 }
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
