@@ -1170,7 +1170,8 @@ extern "C" int frnn_b200_linear_plan(int function, int B, int T, int N, int D, f
   if (B < 1 || T < 1 || N < 1 || D < 1) return -5;
   const long long nd = static_cast<long long>(N) * D;
   const int gates = function == FRNN_LINEAR_LEAKY ? 2 : 4;
-  if (nd * gates > 0x7fffffffLL || T > 0x7fffff00) return -2;  // steps are counted past the end by less than two tiles
+  // the sum of db counts its columns past the end by up to 31, steps are counted so by less than two tiles
+  if (nd * gates > 0x7fffffe0LL || T > 0x7fffff00) return -2;
   const int channels = lin_channels(static_cast<int>(nd));
   const int steps = function == FRNN_LINEAR_LEAKY ? LinCell<FRNN_LINEAR_LEAKY>::kTile : LinCell<FRNN_LINEAR_LSTM>::kTile;
   const long long blocks = B * ((nd + channels - 1) / channels), tiles = (static_cast<long long>(T) + steps - 1) / steps;
