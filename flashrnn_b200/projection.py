@@ -113,10 +113,10 @@ def _product_forward(x, weight, bias, residual, activation, keep: bool):
     rc = lib.frnn_b200_product_forward(
         x.data_ptr(), weight.data_ptr(), _ptr(bias), bias is not None and bias.dtype == torch.bfloat16, _ptr(residual),
         _lib.ACTIVATIONS[activation], y.data_ptr(), _ptr(z), M, J, I, _ptr(work), err, _stream(dev))
+    if word is not None:
+        _launched(word, "frnn_b200_product_forward")   # the tiles have the word, whether the pass behind them was accepted or not
     if rc:
         _lib.check(rc, "frnn_b200_product_forward")
-    if word is not None:
-        _launched(word, "frnn_b200_product_forward")
     return y, z
 
 
