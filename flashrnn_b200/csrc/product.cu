@@ -95,6 +95,12 @@ __device__ __forceinline__ void umma_commit_pair_here(uint32_t bar) {  // ... of
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+// Behind a wait that ran out or was called off: copies in flight land before their buffer is used again or the CTA leaves. From this GPU's
+// memory they take a few microseconds.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -311,10 +317,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         dead = !mbar_wait_bounded<false, true>(smem_u32(&s_empty[s]), r & 1, kLimit, abort_flag);
         if (dead) atomicCAS(p.err, 0, kErrWaitEmpty);
       }
-      if (dead) {  // copies in flight land before the CTA leaves
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
-      }
+      if (dead) settle();
     }
   } else if (warp == kEpiWarps + 1) {
     if (lane == 0 && cta == 0) {
@@ -398,8 +401,7 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
       if (!have) {
         if (lane == 0) {
           atomicCAS(p.err, 0, kErrWaitMma);
-          const uint64_t t0 = global_timer_ns();  // a residual on its way lands before the CTA leaves
-          while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+          settle();  // a residual may be on its way
         }
         break;
       }
@@ -465,7 +467,11 @@ product_kernel(const ProductParams p, const __grid_constant__ CUtensorMap a_map,
         act_row<ACT>(v);
         if (p.has_residual) {
           if (!mbar_wait_warp<false>(smem_u32(&s_res[warp][slot]), (res_phase >> slot) & 1u, kLimit, abort_flag)) {
-            if (lane == 0) atomicCAS(p.err, 0, kErrWaitWx);
+            if (lane == 0) {
+              atomicCAS(p.err, 0, kErrWaitWx);
+              settle();
+            }
+            __syncwarp();
           }
           res_phase ^= 1u << slot;
 #pragma unroll
