@@ -262,7 +262,8 @@ typedef struct frnn_b200_product_plan {
 int frnn_b200_product_plan(int64_t rows, int outputs, int inputs, frnn_b200_product_plan_t* out);
 
 /* bias, residual may be NULL; z: fp16 [rows, outputs], what the backward call takes the activation's slope at, or NULL. y must not
- * overlap an input. */
+ * overlap an input. Waits of either call are bounded (2 s); one that runs out is reported through err as 102 to 105. Test hook for that:
+ * with err[4] = 1 nothing is multiplied, so what waits for the products gives up. */
 int frnn_b200_product_forward(const void* x, const void* w, const void* bias, int bias_bf16, const void* residual, int activation, void* y,
                               void* z, int64_t rows, int outputs, int inputs, float* work, int* err, void* stream);
 
