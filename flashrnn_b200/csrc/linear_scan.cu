@@ -9,7 +9,8 @@
 //
 // Backward: with dc_t the gradient that reaches c_t through hidden_t, g_t = dc_t + f_{t+1} g_{t+1}; the same scan in reverse
 // time over e_t = f_t (dc_t + e_{t+1}). The gates' gradients need c_{t-1}: it is recomputed from Wx, which has to be read
-// anyway, and from the state at the start of every tile, which the forward pass keeps (1/128 of a history).
+// anyway, and from the state at the start of every tile, which the forward pass keeps: 4 bytes per channel and tile, 1/64 (LSTM 1/32) of what the
+// hidden states take in bf16.
 //
 // Few channels: time is cut. One CTA takes a tile of 128 (LSTM: 64) steps x 64 channels of a batch row, read once into registers:
 // a thread has L steps of VEC neighbouring channels, scans them, the tile's spans are joined by shuffles and through shared memory,
@@ -19,11 +20,11 @@
 // depend on timing, so two calls give the same bits. CTAs take their tiles from a counter, earlier steps first: whoever is waited for
 // has started. Many channels, or next to no time: a thread walks its channels through the whole sequence (below).
 //
-// The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. Tiles reach 50 - 60 % of it in bf16 (leaky,
-// B8 T2048 N32 D128: 102 us of 61 forward, 197 of 103 backward) and 83 - 89 % in fp32 (B4 T4096: 138 of 123, 247 of 205): per step and
-// channel 27 instructions (ncu), at 0.5 issued a cycle, in a chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM; more than half of
-// the instructions are the tile's and not the steps', so smaller tiles lose more (64 steps: 132 us) than their shorter chain gains.
-// Walks reach 80 % (leaky, B32 T2048 N32 D128: 309 of 246, 509 of 410).
+// The floor is the bytes: leaky bf16 6 a step and channel forward, 10 backward; lstm 10 and 18. With many channels tiles reach 50 % of it in bf16
+// (leaky, B8 T2048 N32 D128: 120 us of 61 forward, 209 of 103 backward) and 83 - 86 % in fp32 (B4 T4096: 149 of 123, 237 of 205); small
+// layers less (fp32 B13 T333 N2 D200: 9 of 3, 17 of 5). Per step and channel 34 instructions forward (ncu), 0.52 issued a cycle, in a
+// chain of load, scan, two barriers and a fetch from other tiles, with 24 warps to an SM. Walks reach 75 % (leaky, B32 T2048 N32 D128: 331 of
+// 246, 539 of 410).
 #include "../../include/flashrnn_b200.h"
 
 #include "column_sum.cuh"
@@ -253,7 +254,8 @@ __device__ __forceinline__ Vec<N> side_(const Vec<N>& m) {  // p
   for (int i = 0; i < N; ++i) asm("set.le.f32.f32 %0, %1, 0f00000000;" : "=f"(r.v[i]) : "f"(m.v[i]));
   return r;
 }
-// The same, made anew: in a later pass over the steps a register to hold it costs more than the instruction.
+// The same, made anew: in a later pass over the steps a register to hold it costs more than the instruction (the leaky backward tile in bf16
+// spills 268 bytes without this, none with it).
 template <int N>
 __device__ __forceinline__ Vec<N> side_again(const Vec<N>& m) {
   Vec<N> r;
@@ -630,7 +632,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_fwd_kernel(const Lin
   load_bias<CELL, VEC>(p, at.ok, at.ch, bias);
 
   // The LSTM keeps the maps of this thread's steps up to each of them, the leaky cell only the decay of each step: its z's as they came in
-  // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 110 us against 125; with the gates made twice 113; 102 now).
+  // and a third CTA per SM cost less than twice the registers (8 x 2048 x 4096: 120 us; with two CTAs 135, with the gates made twice 135).
   constexpr int MAPS = CELL == FRNN_LINEAR_LSTM ? L : 1, DECAYS = CELL == FRNN_LINEAR_LEAKY ? L : 1;
   V A[MAPS], H[MAPS], decay[DECAYS], a, h;
   auto gates = [&](int l, V& m, V& w) {
@@ -886,12 +888,13 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) linear_bwd_kernel(const Lin
 // Many channels: there is no need to cut time. A thread walks its two channels (one, where ND is odd) through the whole sequence, the
 // next steps' loads in flight while it computes; no exchange, a third of the instructions of a tile. The states it keeps for the
 // backward pass are kWalkSteps apart: what the backward walk recomputes between two of them stays in registers.
-// A step takes 80 - 100 ns (LSTM 190 - 230) however many threads there are, until the memory is full, so it depends on the channels B N D who
-// is faster; walk against tile, forward + backward, us, bf16 and fp32: leaky 65536 x T2048 219 + 353, 199 + 382; 81920 250 + 405, 248 + 476;
-// 131072 310 + 522, 396 + 766; fp32 65536 x T1024 163 + 299, 149 + 258; 98304 232 + 381, 227 + 389; 131072 314 + 472, 299 + 514. LSTM 65536 x T1024
-// 232 + 379, 189 + 379; 98304 397 + 584, 281 + 565; 131072 459 + 663, 376 + 746; fp32 98304 420 + 780, 413 + 708; 131072 495 + 922, 574 + 920.
-// Channels that are no multiple of four have slower tiles: 48960 x T512 59 + 96, 70 + 120 (LSTM 102 + 157, 119 + 226). Up to 16 steps there is
-// nothing to cut: 4 x 1 x 768 2.5 us, 4.9 in a tile.
+// A step takes about 110 ns forward (LSTM 240) however many threads there are, until the memory is full, so it depends on the channels B N D who
+// is faster; walk against tile, forward + backward, us: leaky bf16 65536 x T2048 234 + 378, 235 + 403; 81920 271 + 438, 296 + 504; 131072 331 + 533,
+// 482 + 796; fp32 65536 363 + 488, 291 + 461; 131072 627 + 1003, 572 + 906. LSTM bf16 65536 x T1024 248 + 458, 207 + 413; 98304 430 + 700,
+// 310 + 618; 131072 489 + 833, 414 + 814; 196608 727 + 1245, 623 + 1221; fp32 98304 436 + 794, 481 + 730; 131072 505 + 930, 646 + 968. The border does
+// not know the type: walks win in the leaky cell's bf16 and the LSTM's fp32, tiles in the other two, by up to 25 % forward.
+// Channels that are no multiple of four have slower tiles: 48960 x T512 55 + 91, 68 + 121 (LSTM 110 + 198, 125 + 242; fp32 112 + 268, 131 + 246). Up
+// to 16 steps there is nothing to cut: 4 x 1 x 768 2.5 us, 4.9 in a tile.
 constexpr int kWalkSteps = 8, kWalkThreads = 64;
 constexpr long long kWalkChannels = 65536, kWalkLstmChannels = 131072, kWalkOddChannels = 32768;
 
@@ -932,6 +935,7 @@ struct Walk {
   }
 };
 
+// The LSTM's with one channel a thread is held to six CTAs per SM; left alone it has registers for five (64 x 512 x 765: 162 us, so 110).
 template <int CELL, int VEC, bool BF16>
 __global__ void __launch_bounds__(kWalkThreads, CELL != FRNN_LINEAR_LSTM ? 7 : VEC == 1 ? 6 : 1) linear_fwd_walk_kernel(const LinParams p) {
   using W = Walk<CELL, VEC, BF16>;

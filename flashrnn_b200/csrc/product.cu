@@ -18,9 +18,9 @@
 // order by product_join_kernel, which then has the epilogue. Few rows take product_rows_kernel.
 //
 // Bound: the tensor pipe where K is long. 64 k's of a 256 x 256 tile take 0.40 us (a library product's 0.37): five stages are
-// enough (8192^3: three 1163 us, four 927, five 873, six 872; library 812). Short sums are bound by the epilogue's latency: a tile of 768
-// k's takes 4.8 us, and 8 warps with the bias read per piece took 7 for bias, gelu and z (8192 x 768 x 2048 36.2 us, now 30.9;
-// without an epilogue 24.7, library 23.2). Start and end of the kernel are 4.6 us.
+// enough (8192^3: three 1163 us, four 927, five 873, six 872; library 812). Short sums are bound by the epilogue's latency, hence its sixteen
+// warps and the bias from a register: a tile of 768 k's takes 4.8 us (8192 x 768 x 2048 with bias, gelu and z 30.9 us, without an epilogue
+// 24.7, library 23.2). Start and end of the kernel are 4.6 us.
 #include "../../include/flashrnn_b200.h"
 
 #include "column_sum.cuh"

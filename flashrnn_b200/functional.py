@@ -148,7 +148,8 @@ def _note_stream(ctx, device: torch.device) -> None:
 
 
 def _refuse_capture(ctx) -> None:
-    """In its backward pass: a capture that autograd would make wait for the default stream, which no capture can, ends the process."""
+    """In its backward pass: a capture that autograd would make wait for the default stream, which no capture can, ends the process. Autograd
+    does not tell a node's stream, so a leaf that another operator used first, on the default stream, is not recognised."""
     if _capturing() and any(node.metadata.get("frnn_stream") == 0 for node in _gradient_nodes(ctx)):
         raise RuntimeError("cannot capture this backward pass: an autograd graph of the same inputs, made eagerly on the default stream, "
                            "is alive; let go of its outputs and losses first, or make it on another stream")
