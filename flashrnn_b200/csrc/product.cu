@@ -610,13 +610,14 @@ __global__ void __launch_bounds__(WARPS * 32) product_rows_kernel(const ProductP
 }
 
 // dz = dy act'(z) (not stored where the activation is none: dz = dy), and the columns' sums of a block's rows for dbias.
-constexpr int kSlopeRows = 64;
+constexpr int kSlopeRows = 64, kGridY = 65535;
 template <int ACT>
 __global__ void __launch_bounds__(256) product_slope_kernel(const __nv_bfloat16* __restrict__ dy, const __half* __restrict__ z,
                                                             __nv_bfloat16* __restrict__ dz, float* __restrict__ part, int M, int N) {
   constexpr int kBatch = 4;  // rows of a warp whose loads are in flight together
   __shared__ float s_sum[8][32][9];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.y * 32 + lane) * 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long j0 = (static_cast<long long>(blockIdx.z) * kGridY + blockIdx.y) * 256, j = j0 + lane * 8;  // 256 columns to a block
   const long long m0 = static_cast<long long>(blockIdx.x) * kSlopeRows + warp;
   float sum[8];
 #pragma unroll
@@ -659,7 +660,8 @@ __global__ void __launch_bounds__(256) product_slope_kernel(const __nv_bfloat16*
 #pragma unroll
   for (int e = 0; e < 8; ++e) s_sum[warp][lane][e] = sum[e];
   __syncthreads();
-  const int l = threadIdx.x >> 3, e = threadIdx.x & 7, col = (blockIdx.y * 32 + l) * 8 + e;
+  const int l = threadIdx.x >> 3, e = threadIdx.x & 7;
+  const long long col = j0 + threadIdx.x;
   if (col < N) {
     float v = 0.0f;
 #pragma unroll
@@ -850,8 +852,7 @@ extern "C" int frnn_b200_product_backward(const void* dy, const void* z, const v
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (slopes || dbias != nullptr) {
     const int blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows), cols = (outputs / 8 + 31) / 32;
-    if (cols > 65535) return -2;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(cols));
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(cols < kGridY ? cols : kGridY), static_cast<unsigned>((cols + kGridY - 1) / kGridY));
     const auto* g = static_cast<const __nv_bfloat16*>(dy);
     const auto* h = static_cast<const __half*>(z);
     auto* d = static_cast<__nv_bfloat16*>(dz);
